@@ -464,6 +464,104 @@ int sra_clip_scale_running_f32(const float* M, int64_t k, int64_t d, int64_t ldm
 int sra_bulyan_dba_f32(const float* X, int64_t n, int64_t d, int64_t ldx, int32_t f, int32_t mode, double* out,
                        int32_t* selected, int32_t* status, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- k12-k14: operators of clients that are language models ----
+ * The reference trains its clients one after another on the whole network
+ * (src/simulate.py:150-202); these run the adapters, embeddings and token
+ * losses of all clients at once, reading and writing rows of the clients'
+ * (N, D) matrices.
+ *
+ * Tokens are the rows of one flat batch.  Segment s holds the tokens
+ * [offsets[s], offsets[s + 1]) (device int64, nseg + 1 ascending values) of
+ * slot slots[s] (device int32): the row of the clients' matrices it belongs
+ * to, or -1 for none.  Two segments may share a slot.  Tokens that no segment
+ * covers have no slot.  A slot outside [-1, nslots) or a token id outside the
+ * vocabulary counts as none and is reported by sra_row_fault_count; offsets
+ * outside [0, tokens] are clamped. */
+typedef enum { SRA_F32 = 0, SRA_BF16 = 1, SRA_F16 = 2 } sra_dtype;
+
+/* Largest adapter rank, and most alternatives of sra_token_logprobs. */
+#define SRA_ADAPTER_MAX_RANK 64
+#define SRA_TOKEN_MAX_TOP 32
+
+/* k12: low-rank adapters beside a shared projection.  Slot c's adapter is
+ * A_c (rank x k) at A + c * lda and B_c (m x rank) at B + c * ldb, row-major
+ * (elements of wdtype: SRA_F32 or dtype).  For token t of slot c
+ *   h_t = A_c x_t,   out_t = base_t + scale * B_c h_t
+ * and out_t = base_t where t has no slot.  x, base and out have dtype; base
+ * may be NULL (zeros) or equal out (in place, same row stride).  hidden
+ * (optional, tokens x rank float32) receives h (0 without a slot).  Sums are
+ * float32.  1 <= rank <= SRA_ADAPTER_MAX_RANK. */
+int sra_adapter_workspace_bytes(int64_t tokens, int64_t k, int64_t m, int32_t rank, int32_t nslots, size_t* bytes);
+int sra_adapter_apply(const void* base, int64_t ldbase, const void* x, int64_t ldx, const void* A, int64_t lda,
+                      const void* B, int64_t ldb, const int64_t* offsets, const int32_t* slots, int32_t nseg,
+                      int64_t tokens, int32_t nslots, int64_t k, int64_t m, int32_t rank, float scale,
+                      int32_t dtype, int32_t wdtype, void* out, int64_t ldo, float* hidden, void* ws,
+                      size_t ws_bytes, void* stream);
+
+/* Its backward pass.  dout (tokens x m, dtype) is the gradient of out; hidden
+ * is sra_adapter_apply's, or NULL to compute it again.
+ *   z_t = B_c' dout_t,   dx_t = dxbase_t + scale * A_c' z_t
+ *   dA_c = scale * sum_t z_t x_t',   dB_c = scale * sum_t dout_t h_t'
+ * dx (dtype), dA (float32, slot stride ldda) and dB (float32, slot stride
+ * lddb) are each optional (NULL); dxbase may be NULL (zeros) or equal dx.
+ * Every slot of dA and dB is written, zeros where a slot has no token;
+ * accumulate != 0 adds to them instead.  No atomics: results do not depend on
+ * the order in which workgroups run. */
+int sra_adapter_grad(const void* dout, int64_t lddo, const void* x, int64_t ldx, const void* A, int64_t lda,
+                     const void* B, int64_t ldb, const int64_t* offsets, const int32_t* slots, int32_t nseg,
+                     int64_t tokens, int32_t nslots, int64_t k, int64_t m, int32_t rank, float scale,
+                     int32_t dtype, int32_t wdtype, const float* hidden, const void* dxbase, int64_t lddxb,
+                     void* dx, int64_t lddx, float* dA, int64_t ldda, float* dB, int64_t lddb,
+                     int32_t accumulate, void* ws, size_t ws_bytes, void* stream);
+
+/* k13: embedding lookup with scaling.  Slot c's table (vocab x dim, row-major,
+ * tdtype) starts at table + c * ldt; offsets = slots = NULL reads slot 0 for
+ * every token.  out_t = scale * table_c[ids[t]] rounded once to odtype; zeros
+ * for a token without a slot. */
+int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const int64_t* ids, const int64_t* offsets,
+              const int32_t* slots, int32_t nseg, int64_t tokens, int32_t nslots, int64_t vocab, int64_t dim,
+              float scale, void* out, int64_t ldo, int32_t odtype, void* stream);
+
+/* Its gradient by sorted tokens: grad_c[v] = scale * sum of dout_t over the
+ * tokens t of slot c with ids[t] = v, t ascending, in float32; grad is float32
+ * with slot stride ldg.  Tokens with ids[t] = padding (pass -1 for none) are
+ * left out.  Every row is written, zeros where no token reads it; accumulate
+ * != 0 adds to the rows that tokens read and leaves the others alone.
+ * nslots * vocab < 2^32 - 1, tokens < 2^31. */
+int sra_embed_grad_workspace_bytes(int64_t tokens, int64_t dim, size_t* bytes);
+int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t* ids, const int64_t* offsets,
+                   const int32_t* slots, int32_t nseg, int64_t tokens, int32_t nslots, int64_t vocab, int64_t dim,
+                   float scale, int64_t padding, float* grad, int64_t ldg, int32_t accumulate, void* ws,
+                   size_t ws_bytes, void* stream);
+
+/* k14: log probabilities of given tokens.  For row x of the rows x vocab
+ * logits (dtype, row stride ldl), with lse = log sum_i exp(x_i):
+ *   logp = x[target] - lse,  entropy = lse - sum_i p_i x_i,
+ * and the top largest logits as (top_logp, top_ids), descending, the lowest
+ * index first among equals, NaN above everything.  entropy (optional), lse,
+ * logp: rows floats; top_logp / top_ids: rows x top, 0 <= top <=
+ * min(vocab, SRA_TOKEN_MAX_TOP).  -inf logits have p = 0 and add nothing to
+ * the entropy; a row of only -inf, or with +inf or NaN, gives NaN.  A target
+ * equal to ignore gives logp 0; one outside the vocabulary gives NaN and is
+ * counted as a row fault.
+ * With grad (rows x vocab, dtype, row stride ldg; may equal logits) it also
+ * writes the logits' gradient for given row gradients of logp and entropy:
+ *   grad_i = grad_logp * (1[i = target] - p_i) - grad_entropy * p_i (log p_i + entropy)
+ * (no logp part for an ignored target; grad_entropy may be NULL), which reads
+ * the logits from memory once for both. */
+int sra_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top, size_t* bytes);
+int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
+                       int64_t vocab, int64_t ignore, int32_t top, float* logp, float* entropy, float* lse,
+                       float* top_logp, int64_t* top_ids, const float* grad_logp, const float* grad_entropy,
+                       void* grad, int64_t ldg, void* ws, size_t ws_bytes, void* stream);
+
+/* The same gradient from a forward pass's lse and entropy (entropy is needed
+ * with grad_entropy only). */
+int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
+                            int64_t vocab, int64_t ignore, const float* lse, const float* entropy,
+                            const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

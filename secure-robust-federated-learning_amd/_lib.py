@@ -125,6 +125,22 @@ _SIGS = {
     "sra_clip_scale_running_f32": [_ptr, _i64, _i64, _i64, _ptr, ctypes.POINTER(_i64), _i32, _dbl, _ptr, _ptr, _ptr,
                                    _sz, _ptr],
     "sra_bulyan_dba_f32": [_ptr, _i64, _i64, _i64, _i32, _i32, _ptr, _ptr, _ptr, _ptr, _sz, _ptr],
+    "sra_adapter_workspace_bytes": [_i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_sz)],
+    "sra_adapter_apply": [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64,
+                          _i32, ctypes.c_float, _i32, _i32, _ptr, _i64, _ptr, _ptr, _sz, _ptr],
+    "sra_adapter_grad": [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64,
+                         _i32, ctypes.c_float, _i32, _i32, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64,
+                         _i32, _ptr, _sz, _ptr],
+    "sra_embed": [_ptr, _i64, _i32, _ptr, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64, ctypes.c_float, _ptr, _i64,
+                  _i32, _ptr],
+    "sra_embed_grad_workspace_bytes": [_i64, _i64, ctypes.POINTER(_sz)],
+    "sra_embed_grad": [_ptr, _i64, _i32, _ptr, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64, ctypes.c_float, _i64,
+                       _ptr, _i64, _i32, _ptr, _sz, _ptr],
+    "sra_token_logprobs_workspace_bytes": [_i64, _i64, _i32, ctypes.POINTER(_sz)],
+    "sra_token_logprobs": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                           _ptr, _ptr, _i64, _ptr, _sz, _ptr],
+    "sra_token_logprobs_grad": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64,
+                                _ptr],
 }
 _RESTYPES = {"sra_last_error": ctypes.c_char_p}
 

@@ -1,5 +1,5 @@
 // Library-wide entry points: error text, version, build limits.
-#include "sra_common.hpp"
+#include "lm_common.hpp"
 
 namespace sra {
 
@@ -22,6 +22,8 @@ extern "C" int sra_max_register_clients(void) { return 128; }
 
 extern "C" int sra_row_fault_count(int32_t reset, uint32_t* count) {
   SRA_REQUIRE(count != nullptr, SRA_ERR_ARG, "null count pointer");
-  *count = sra::krum_row_faults(reset != 0) + sra::bulyan_row_faults(reset != 0);
+  const bool r = reset != 0;
+  *count = sra::krum_row_faults(r) + sra::bulyan_row_faults(r) + sra::adapter_row_faults(r) +
+           sra::embed_row_faults(r) + sra::logprob_row_faults(r);
   return SRA_OK;
 }

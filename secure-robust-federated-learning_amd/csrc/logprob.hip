@@ -1,0 +1,494 @@
+// k14 — log probabilities of given tokens, with the entropy and the top
+// alternatives of every row, and the logits' gradient.
+//
+// One pass over a row keeps, per thread, the running maximum m and
+//   s = sum e^{x - m},   u = sum e^{x - m} (x - m),
+// joined over threads, waves and (for few long rows) workgroups by
+//   (m, s, u) + (m', s', u'):  with M = max(m, m'), d = m - M, f = e^d:
+//   s f + ...,  (u + s d) f + ...
+// so that  lse = m + log s,  logp = x_target - lse,  entropy = log s - u / s
+// without a difference of large numbers.
+#include "lm_common.hpp"
+
+namespace sra {
+
+unsigned int logprob_row_faults(bool reset) { return tu_row_faults(reset); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
+// differences from the maximum below this have e^d = 0; clamping them keeps
+// 0 * d from becoming NaN for -inf logits
+constexpr float kFarBelow = -1.0e4f;
+
+__device__ __forceinline__ float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+struct Stats {
+  float m, s, u;
+};
+
+__device__ __forceinline__ void rescale(Stats& a, float M) {
+  const float d = a.m - M;
+  const float f = fast_exp(d);
+  a.u = (a.u + a.s * fmaxf(d, kFarBelow)) * f;
+  a.s *= f;
+  a.m = M;
+}
+
+__device__ __forceinline__ void join(Stats& a, Stats b) {
+  const float M = __builtin_elementwise_maximum(a.m, b.m);   // keeps a NaN
+  rescale(a, M);
+  rescale(b, M);
+  a.s += b.s;
+  a.u += b.u;
+}
+
+template <int N>
+__device__ __forceinline__ void add_values(Stats& a, const float (&x)[N], float mx) {
+  if (!(mx <= a.m)) rescale(a, __builtin_elementwise_maximum(a.m, mx));
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float d = x[e] - a.m;
+    const float p = fast_exp(d);
+    a.s += p;
+    a.u += p * fmaxf(d, kFarBelow);
+  }
+}
+
+__device__ __forceinline__ Stats wave_join(Stats a) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const Stats b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)};
+    join(a, b);
+  }
+  return a;
+}
+
+// ---------------------------------------------------------------------------
+// The largest logits.  Lane j < k of a wave holds the j-th best (key, index).
+// Keys order floats as unsigned integers: -0 equals +0, NaN above everything,
+// 0 is no entry; equal keys order by the lower index.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ unsigned key_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+  const unsigned b = (key & 0x80000000u) ? (key & 0x7fffffffu) : ~key;
+  return __builtin_bit_cast(float, b);      // the NaN key maps to a NaN
+}
+
+struct Top {
+  unsigned key;
+  int idx;
+  unsigned kth;      // the k-th best's key and index, the same in every lane
+  int kth_idx;
+  float thr;         // its value; a new x with x <= thr cannot enter
+};
+
+__device__ __forceinline__ bool before(unsigned ka, int ia, unsigned kb, int ib) {
+  return ka > kb || (ka == kb && ia < ib);
+}
+
+__device__ __forceinline__ void top_clear(Top& t) {
+  t.key = t.kth = 0;
+  t.idx = t.kth_idx = 0x7fffffff;
+  t.thr = -__builtin_inff();
+}
+
+__device__ __forceinline__ void top_insert(Top& t, int k, unsigned key, int idx) {
+  const int lane = threadIdx.x & 63;
+  const unsigned pk = __shfl_up(t.key, 1);
+  const int pi = __shfl_up(t.idx, 1);
+  if (lane < k && !before(t.key, t.idx, key, idx)) {
+    const bool prev = lane > 0 && !before(pk, pi, key, idx);
+    t.key = prev ? pk : key;
+    t.idx = prev ? pi : idx;
+  }
+  t.kth = __shfl(t.key, k - 1);
+  t.kth_idx = __shfl(t.idx, k - 1);
+  t.thr = t.kth == 0 ? -__builtin_inff() : value_of(t.kth);
+}
+
+// Put what belongs there of every lane's N values: the wave's best remaining
+// one at a time, so that at most k insertions follow whatever the order.
+template <int N, typename Index>
+__device__ __forceinline__ void top_offer(Top& t, int k, const unsigned (&key)[N], Index&& index, unsigned live) {
+  while (true) {
+    unsigned bk = 0;
+    int bi = 0x7fffffff, be = -1;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if ((live >> e & 1u) && before(key[e], index(e), bk, bi)) {
+        bk = key[e];
+        bi = index(e);
+        be = e;
+      }
+    const int own = bi;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned ok = __shfl_xor(bk, o);
+      const int oi = __shfl_xor(bi, o);
+      if (before(ok, oi, bk, bi)) {
+        bk = ok;
+        bi = oi;
+      }
+    }
+    if (bk == 0 || !before(bk, bi, t.kth, t.kth_idx)) return;
+    top_insert(t, k, bk, bi);
+    if (be >= 0 && own == bi) live &= ~(1u << be);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Walk a row in index order: f(x[8], first index, valid) per lane, wave w of
+// nw taking every nw-th stretch of 512 from `from` to `to`.  16-byte loads from
+// the first aligned element on; the few elements before it and after the last
+// whole stretch go one by one through the same call.
+// ---------------------------------------------------------------------------
+constexpr int kPer = 8;
+constexpr int kStretch = 64 * kPer;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[kPer]) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = a[e];
+      x[4 + e] = b[e];
+    }
+  } else {
+    union {
+      u32x4 v;
+      T t[kPer];
+    } q;
+    q.v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = to_f32(q.t[e]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[kPer]) {
+  if constexpr (sizeof(T) == 4) {
+    f32x4 a, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = x[e];
+      b[e] = x[4 + e];
+    }
+    reinterpret_cast<f32x4*>(p)[0] = a;
+    reinterpret_cast<f32x4*>(p)[1] = b;
+  } else {
+    union {
+      u32x4 v;
+      T t[kPer];
+    } q;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) q.t[e] = from_f32<T>(x[e]);
+    *reinterpret_cast<u32x4*>(p) = q.v;
+  }
+}
+
+// elements before the first 16-byte aligned one
+template <typename T>
+__device__ __forceinline__ int head_of(const T* row, int64_t n) {
+  const int h = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T));
+  return static_cast<int>(min(static_cast<int64_t>(h), n));
+}
+
+template <typename T, typename F>
+__device__ __forceinline__ void walk(const T* row, int from, int to, int w, int nw, F&& f) {
+  const int lane = threadIdx.x & 63;
+  const int h = from + head_of(row + from, to - from);
+  float x[kPer];
+  if (w == 0 && h > from) {                      // at most 7 elements, one a lane
+    const bool in = from + lane < h;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = -__builtin_inff();
+    if (in) x[0] = to_f32(row[from + lane]);
+    f(x, from + lane, in ? 1 : 0);
+  }
+  const int body = (to - h) / kStretch;
+  for (int b = w; b < body; b += nw) {
+    const int i = h + b * kStretch + lane * kPer;
+    load8(row + i, x);
+    f(x, i, kPer);
+  }
+  const int t0 = h + body * kStretch;
+  if (t0 < to && body % nw == w) {               // the last, partial stretch
+    const int i = t0 + lane * kPer;
+    const int valid = max(0, min(kPer, to - i));
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = e < valid ? to_f32(row[i + e]) : -__builtin_inff();
+    f(x, i, valid);
+  }
+}
+
+struct Args {
+  int64_t ldl;
+  const int64_t* targets;
+  int64_t rows;
+  int vocab;
+  int64_t ignore;
+  int top;
+  float* logp;
+  float* entropy;
+  float* lse;
+  float* top_logp;
+  int64_t* top_ids;
+  const float* grad_logp;
+  const float* grad_entropy;
+  int64_t ldg;
+};
+
+// the gradient of one row, given its lse and entropy
+template <typename T>
+__device__ __forceinline__ void grad_row(const T* row, T* grow, int vocab, int64_t target, float lse, float ent,
+                                         float gl, float ge, int w, int nw) {
+  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
+  walk(row, 0, vocab, w, nw, [&](float (&x)[kPer], int i, int valid) {
+    float g[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float l = x[e] - lse;
+      const float p = fast_exp(l);
+      float v = -gl * p;
+      if (ge != 0.f) v -= ge * p * (fmaxf(l, kFarBelow) + ent);
+      if (i + e == target) v += gl;
+      g[e] = v;
+    }
+    if (valid == kPer && same) {
+      store8(grow + i, g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (e < valid) grow[i + e] = from_f32<T>(g[e]);
+    }
+  });
+}
+
+// WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.
+template <typename T, int WAVES, bool TOP, bool GRAD>
+__global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
+    logprob_kernel(const T* logits, Args a, T* grad) {
+  static_assert(WAVES == 1 || WAVES >= 4, "a workgroup's waves share the barrier of one row");
+  constexpr int kRows = WAVES < 4 ? 4 / WAVES : 1;
+  __shared__ Stats sh_stats[kRows * WAVES];
+  __shared__ unsigned sh_key[TOP ? kRows * WAVES * SRA_TOKEN_MAX_TOP : 1];
+  __shared__ int sh_idx[TOP ? kRows * WAVES * SRA_TOKEN_MAX_TOP : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int local = wave / WAVES, w = wave % WAVES;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + local;
+  const bool live = r < a.rows;
+
+  Stats st{kLowest, 0.f, 0.f};
+  Top t;
+  top_clear(t);
+  const T* row = logits + (live ? r : 0) * a.ldl;
+  if (live) {
+    walk(row, 0, a.vocab, w, WAVES, [&](float (&x)[kPer], int i, int valid) {
+      float mx = x[0];
+#pragma unroll
+      for (int e = 1; e < kPer; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
+      add_values(st, x, mx);
+      if constexpr (TOP) {
+        if (__ballot(t.kth == 0 || !(mx <= t.thr)) != 0) {
+          unsigned key[kPer];
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) key[e] = key_of(x[e]);
+          top_offer(t, a.top, key, [&](int e) { return i + e; }, (1u << valid) - 1u);
+        }
+      }
+    });
+  }
+  st = wave_join(st);
+  if constexpr (WAVES > 1) {
+    if (lane == 0) sh_stats[wave] = st;
+    if constexpr (TOP) {
+      if (lane < a.top) {
+        sh_key[wave * SRA_TOKEN_MAX_TOP + lane] = t.key;
+        sh_idx[wave * SRA_TOKEN_MAX_TOP + lane] = t.idx;
+      }
+    }
+    __syncthreads();
+    // every wave joins them in the same order
+    st = sh_stats[local * WAVES];
+    for (int q = 1; q < WAVES; ++q) join(st, sh_stats[local * WAVES + q]);
+    if constexpr (TOP) {
+      if (w == 0)
+        for (int q = 1; q < WAVES; ++q) {
+          const unsigned key[1] = {lane < a.top ? sh_key[(wave + q) * SRA_TOKEN_MAX_TOP + lane] : 0u};
+          const int idx = lane < a.top ? sh_idx[(wave + q) * SRA_TOKEN_MAX_TOP + lane] : 0x7fffffff;
+          top_offer(t, a.top, key, [&](int) { return idx; }, 1u);
+        }
+    }
+  }
+  if (!live) return;
+  const float ls = logf(st.s);
+  const float lse = st.m + ls;
+  const float ent = ls - st.u / st.s;
+  const int64_t target = a.targets[r];
+  const bool ignored = target == a.ignore;
+  const bool bad = !ignored && (target < 0 || target >= a.vocab);
+  if (w == 0 && lane == 0) {
+    float lp = 0.f;
+    if (bad) {
+      count_row_fault();
+      lp = __builtin_nanf("");
+    } else if (!ignored) {
+      lp = to_f32(row[target]) - lse;
+    }
+    a.logp[r] = lp;
+    a.lse[r] = lse;
+    if (a.entropy != nullptr) a.entropy[r] = ent;
+  }
+  if constexpr (TOP) {
+    if (w == 0 && lane < a.top) {
+      a.top_logp[r * a.top + lane] = value_of(t.key) - lse;
+      a.top_ids[r * a.top + lane] = t.idx;
+    }
+  }
+  if constexpr (GRAD) {
+    // the target is read before an in-place gradient replaces it
+    if constexpr (WAVES > 1) __syncthreads(); else __threadfence_block();
+    const float gl = ignored || bad ? 0.f : a.grad_logp[r];
+    const float ge = a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f;
+    grad_row(row, grad + r * a.ldg, a.vocab, ignored || bad ? -1 : target, lse, ent, gl, ge, w, WAVES);
+  }
+}
+
+// the gradient from a forward pass's lse and entropy: 4 waves take a stretch of
+// 8192 of a row
+constexpr int kGradSpan = 8192;
+
+template <typename T>
+__global__ void __launch_bounds__(256) logprob_grad_kernel(const T* logits, Args a, const float* __restrict__ lse,
+                                                           const float* __restrict__ entropy, T* grad) {
+  const int64_t r = blockIdx.x;
+  const int from = blockIdx.y * kGradSpan;
+  const int n = min(kGradSpan, a.vocab - from);
+  int64_t target = a.targets[r];
+  float gl = a.grad_logp[r];
+  const bool ignored = target == a.ignore;
+  if (ignored || target < 0 || target >= a.vocab) {
+    if (!ignored && from == 0 && threadIdx.x == 0) count_row_fault();
+    gl = 0.f;
+    target = -1;
+  }
+  const float ge = a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f;
+  const float ent = a.grad_entropy != nullptr ? entropy[r] : 0.f;
+  grad_row(logits + r * a.ldl + from, grad + r * a.ldg + from, n, target - from, lse[r], ent, gl, ge,
+           threadIdx.x >> 6, 4);
+}
+
+static int check_logits(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
+                        int64_t vocab) {
+  if (int rc = check_dtype(dtype, "dtype")) return rc;
+  SRA_REQUIRE(rows >= 0 && rows < (int64_t{1} << 31), SRA_ERR_SHAPE, "rows must be in [0, 2^31), got %lld",
+              static_cast<long long>(rows));
+  SRA_REQUIRE(vocab >= 1 && vocab < (int64_t{1} << 28), SRA_ERR_SHAPE, "vocab must be in [1, 2^28), got %lld",
+              static_cast<long long>(vocab));
+  SRA_REQUIRE(rows == 0 || (logits != nullptr && targets != nullptr), SRA_ERR_ARG,
+              "logits and targets must be non-null");
+  SRA_REQUIRE(rows <= 1 || ldl >= vocab, SRA_ERR_SHAPE, "logits need a row stride >= %lld, got %lld",
+              static_cast<long long>(vocab), static_cast<long long>(ldl));
+  SRA_REQUIRE((reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype)) == 0, SRA_ERR_ARG,
+              "logits are not aligned to their type");
+  return SRA_OK;
+}
+
+static int check_grad(const void* logits, int64_t ldl, const void* grad, int64_t ldg, int64_t rows, int64_t vocab,
+                      int32_t dtype) {
+  SRA_REQUIRE(rows <= 1 || ldg >= vocab, SRA_ERR_SHAPE, "grad needs a row stride >= %lld, got %lld",
+              static_cast<long long>(vocab), static_cast<long long>(ldg));
+  SRA_REQUIRE(grad != logits || ldg == ldl || rows <= 1, SRA_ERR_SHAPE,
+              "logits and grad are one buffer with two row strides");
+  SRA_REQUIRE((reinterpret_cast<uintptr_t>(grad) % dtype_size(dtype)) == 0, SRA_ERR_ARG,
+              "grad is not aligned to its type");
+  return SRA_OK;
+}
+
+template <typename T, int WAVES>
+static int launch_rows(const void* logits, const Args& a, void* grad, hipStream_t st) {
+  constexpr int kRows = WAVES < 4 ? 4 / WAVES : 1;
+  const dim3 grid(static_cast<unsigned>(cdiv(a.rows, kRows))), block(WAVES < 4 ? 256 : WAVES * 64);
+  const T* l = static_cast<const T*>(logits);
+  T* g = static_cast<T*>(grad);
+  if (a.top > 0 && g != nullptr)
+    hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, true>), grid, block, 0, st, l, a, g);
+  else if (a.top > 0)
+    hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, false>), grid, block, 0, st, l, a, g);
+  else if (g != nullptr)
+    hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, true>), grid, block, 0, st, l, a, g);
+  else
+    hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, false>), grid, block, 0, st, l, a, g);
+  return launch_status("logprob_kernel");
+}
+
+template <typename F>
+static int with_type(int32_t dtype, F&& f) {
+  if (dtype == SRA_F32) return f(float{});
+  if (dtype == SRA_BF16) return f(__bf16{});
+  return f(_Float16{});
+}
+
+}  // namespace sra
+
+using namespace sra;
+
+extern "C" int sra_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top, size_t* bytes) {
+  SRA_REQUIRE(bytes != nullptr, SRA_ERR_ARG, "null bytes pointer");
+  SRA_REQUIRE(rows >= 0 && vocab >= 1 && top >= 0, SRA_ERR_SHAPE, "rows, vocab and top must not be negative");
+  *bytes = 16;
+  return SRA_OK;
+}
+
+extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                  int64_t rows, int64_t vocab, int64_t ignore, int32_t top, float* logp,
+                                  float* entropy, float* lse, float* top_logp, int64_t* top_ids,
+                                  const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
+                                  void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_logits(logits, ldl, dtype, targets, rows, vocab)) return rc;
+  SRA_REQUIRE(top >= 0 && top <= vocab, SRA_ERR_ARG, "top must be in [0, vocab], got %d", top);
+  SRA_REQUIRE(top <= SRA_TOKEN_MAX_TOP, SRA_ERR_UNSUPPORTED, "top %d is above %d", top, SRA_TOKEN_MAX_TOP);
+  SRA_REQUIRE(rows == 0 || (logp != nullptr && lse != nullptr), SRA_ERR_ARG, "logp and lse must be non-null");
+  SRA_REQUIRE(rows == 0 || top == 0 || (top_logp != nullptr && top_ids != nullptr), SRA_ERR_ARG,
+              "top_logp and top_ids must be non-null");
+  SRA_REQUIRE(grad == nullptr || grad_logp != nullptr, SRA_ERR_ARG, "the gradient needs grad_logp");
+  if (grad != nullptr)
+    if (int rc = check_grad(logits, ldl, grad, ldg, rows, vocab, dtype)) return rc;
+  size_t need = 0;
+  if (int rc = sra_token_logprobs_workspace_bytes(rows, vocab, top, &need)) return rc;
+  SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "token_logprobs workspace: need %zu bytes, got %zu",
+              need, ws_bytes);
+  if (rows == 0) return SRA_OK;
+  const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, top, logp, entropy, lse, top_logp, top_ids,
+               grad_logp, grad_entropy, ldg};
+  return with_type(dtype, [&](auto t) {
+    return launch_rows<decltype(t), 4>(logits, a, grad, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                       int64_t rows, int64_t vocab, int64_t ignore, const float* lse,
+                                       const float* entropy, const float* grad_logp, const float* grad_entropy,
+                                       void* grad, int64_t ldg, void* stream) {
+  if (int rc = check_logits(logits, ldl, dtype, targets, rows, vocab)) return rc;
+  if (rows == 0) return SRA_OK;
+  SRA_REQUIRE(lse != nullptr && grad_logp != nullptr && grad != nullptr, SRA_ERR_ARG,
+              "lse, grad_logp and grad must be non-null");
+  SRA_REQUIRE(grad_entropy == nullptr || entropy != nullptr, SRA_ERR_ARG,
+              "grad_entropy needs the forward pass's entropy");
+  if (int rc = check_grad(logits, ldl, grad, ldg, rows, vocab, dtype)) return rc;
+  const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, 0, nullptr, nullptr, nullptr, nullptr, nullptr,
+               grad_logp, grad_entropy, ldg};
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(cdiv(vocab, kGradSpan)));
+    hipLaunchKernelGGL((logprob_grad_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const T*>(logits), a, lse, entropy, static_cast<T*>(grad));
+    return launch_status("logprob_grad_kernel");
+  });
+}

@@ -104,16 +104,20 @@ class ClientStore:
     def record(self, c):
         """Client ``c`` finished local training: write its update into row c and
         restore the parameters from the snapshot (simulate.py:187-199)."""
+        self._record(c, self._table())
+
+    def _record(self, c, table):
+        """``record`` with the client's parameters where ``table`` says."""
         c = int(c)
         if not 0 <= c < self.nworker:
             raise IndexError("client %d out of range [0, %d)" % (c, self.nworker))
         row = self.U[c]
         if self.momentum:
             self._sync_row(c)   # the momentum reads local_grads[c] as the caller left it
-            _lib.call("sra_record_momentum_f64", *self._table(), self.snap.data_ptr(), self.one_minus_beta,
+            _lib.call("sra_record_momentum_f64", *table, self.snap.data_ptr(), self.one_minus_beta,
                       self.beta, row.data_ptr(), self._stream())
         else:
-            _lib.call("sra_record_delta_f32", *self._table(), self.snap.data_ptr(), row.data_ptr(), self._stream())
+            _lib.call("sra_record_delta_f32", *table, self.snap.data_ptr(), row.data_ptr(), self._stream())
         # the reference assigns fresh arrays to local_grads[c][idx]
         self.local_grads[c] = list(self._views[c])
 
@@ -166,21 +170,85 @@ class ClientStore:
             raise TypeError("aggregate must be float32 or float64, got %s" % flat.dtype)
 
 
-def fl_round(network, store, choices, local_update, args, state=None, attack="noattack", mal_index=()):
+class ClientBank:
+    """Every chosen client's own parameters and gradients for a round, as rows of
+    two (n, D) float32 device matrices laid out like the store's updates, so that
+    all of them train at once (``lm``) instead of one after another on the one
+    network (simulate.py:150-202).
+
+    Row i belongs to the i-th chosen client: ``param(l)`` and ``grad(l)`` are the
+    (n, *shape) views of layer l that ``lm.adapter_apply``, ``lm.embed`` and their
+    gradients take, with i as the slot."""
+
+    def __init__(self, store, n):
+        self.store = store
+        self.n = int(n)
+        if not 1 <= self.n <= store.nworker:
+            raise ValueError("a bank holds 1 to %d clients, got %d" % (store.nworker, self.n))
+        self.P = torch.empty((self.n, store.D), dtype=torch.float32, device=store.device)
+        self.G = torch.zeros_like(self.P)
+        self.choices = None
+        rows = self.P.data_ptr() + 4 * store.D * np.arange(self.n, dtype=np.uint64)
+        self._ptrs = torch.tensor(rows.astype(np.uint64).view(np.int64), device=store.device)
+        self._seg = torch.tensor([0, store.D], dtype=torch.int64, device=store.device)
+
+    def _view(self, X, l):
+        s = self.store
+        return X[:, s.seg[l]:s.seg[l + 1]].view((self.n,) + s.shapes[l])
+
+    def param(self, l):
+        return self._view(self.P, l)
+
+    def grad(self, l):
+        return self._view(self.G, l)
+
+    def load(self, choices):
+        """Every chosen client starts from the snapshot (simulate.py:146-148)."""
+        choices = [int(c) for c in choices]
+        if len(choices) != self.n or len(set(choices)) != self.n:
+            raise ValueError("this bank holds %d different clients, got %r" % (self.n, choices))
+        for c in choices:
+            if not 0 <= c < self.store.nworker:
+                raise IndexError("client %d out of range [0, %d)" % (c, self.store.nworker))
+        self.choices = choices
+        self.P.copy_(self.store.snap.expand_as(self.P))
+        self.G.zero_()
+
+    def step(self, lr):
+        """One SGD step of every client."""
+        self.P.add_(self.G, alpha=-float(lr))
+
+    def record(self):
+        """Every client's update into its row of the store (simulate.py:187-199);
+        the bank's rows are back at the snapshot afterwards."""
+        if self.choices is None:
+            raise RuntimeError("load the round's choices before recording")
+        for i, c in enumerate(self.choices):
+            self.store._record(c, (self._ptrs.data_ptr() + 8 * i, self._seg.data_ptr(), 1, self.store.D))
+
+
+def fl_round(network, store, choices, local_update, args, state=None, attack="noattack", mal_index=(), bank=None):
     """One round of simulate.py's loop (:139-404) with device-resident updates.
 
     ``local_update(c)`` runs client c's local training on ``network`` (the
     reference's inner loops, :175-186); the store records the update and
-    restores the parameters.  ``attack`` is one of the reference's post-training
+    restores the parameters.  With a ``ClientBank`` of len(choices) clients,
+    ``local_update(bank)`` trains them all at once on the bank's rows instead.
+    ``attack`` is one of the reference's post-training
     attacks (:218-229: ``trimmedmean`` with b=1.5, ``krum`` per layer, ``xie``),
     run on the device by ``srfl_amd.attack``.  The aggregate is subtracted from
     the parameters in place and returned as the flat (D,) device vector."""
     from . import attack as atk, dispatch
 
     store.snapshot()
-    for c in choices:
-        local_update(int(c))
-        store.record(int(c))
+    if bank is not None:
+        bank.load(choices)
+        local_update(bank)
+        bank.record()
+    else:
+        for c in choices:
+            local_update(int(c))
+            store.record(int(c))
     lg = store.local_grads
     if attack == "trimmedmean":
         atk.attack_trimmedmean(network, lg, mal_index, b=1.5)

@@ -160,7 +160,8 @@ def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=Fal
     x (T, K) and base (T, M) are activations of one type (float32, bfloat16,
     float16); base None means zeros.  A (n, r, K) and B (n, M, r) are float32 (rows
     of the clients' matrix) or the activations' type, 1 <= r <= 64.  Tokens without
-    a slot get base.  ``out`` may be base (in place).  hidden=True also returns the
+    a slot get base.  An infinite operand makes its products infinite or NaN.
+    ``out`` may be base (in place).  hidden=True also returns the
     float32 (T, r) products A x for ``adapter_grad``."""
     head, keep, T, K, M, n, r, dtype, wdtype = _adapter_args(x, A, B, offsets, slots)
     dev = x.device

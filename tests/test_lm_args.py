@@ -50,7 +50,7 @@ def test_adapter_workspace_refuses():
     (dict(dout=None), ValueError, "dout"), (dict(lddo=63), ValueError, "stride"), (dict(lddx=63), ValueError, "stride"),
     (dict(ldda=511), ValueError, "slot strides"), (dict(lddb=511), ValueError, "slot strides"),
     (dict(rank=65), NotImplementedError, "rank"), (dict(ws_bytes=8), ValueError, "workspace"),
-    (dict(lddxb=70), ValueError, "one buffer"),
+    (dict(lddxb=70), ValueError, "one buffer"), (dict(nslots=65536), NotImplementedError, "65535"),
 ])
 def test_adapter_grad_refuses(kw, exc, match):
     a = dict(dout=P, lddo=64, x=P, ldx=64, A=P, lda=512, B=P, ldb=512, offsets=P, slots=P, nseg=2, tokens=8, nslots=4,

@@ -125,7 +125,7 @@ _SIGS = {
     "sra_clip_scale_running_f32": [_ptr, _i64, _i64, _i64, _ptr, ctypes.POINTER(_i64), _i32, _dbl, _ptr, _ptr, _ptr,
                                    _sz, _ptr],
     "sra_bulyan_dba_f32": [_ptr, _i64, _i64, _i64, _i32, _i32, _ptr, _ptr, _ptr, _ptr, _sz, _ptr],
-    "sra_adapter_workspace_bytes": [_i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_sz)],
+    "sra_adapter_workspace_bytes": [_i64, _i32, _i32, _i64, _i64, _i32, ctypes.POINTER(_sz)],
     "sra_adapter_apply": [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64,
                           _i32, ctypes.c_float, _i32, _i32, _ptr, _i64, _ptr, _ptr, _sz, _ptr],
     "sra_adapter_grad": [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64,

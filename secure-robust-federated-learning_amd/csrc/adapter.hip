@@ -35,52 +35,79 @@ unsigned int adapter_row_faults(bool reset) { return tu_row_faults(reset); }
 // ---------------------------------------------------------------------------
 // 8 values a lane, and their products
 // ---------------------------------------------------------------------------
-template <typename S>
-struct Raw8 {
-  S v[8];
+template <typename S, int N>
+struct RawN {
+  S v[N];
 };
+template <typename S>
+using Raw8 = RawN<S, 8>;
+template <typename S>
+using Raw4 = RawN<S, 4>;
 
-// 8 consecutive elements at any alignment of their type (the hardware's global
-// loads take it); valid < 8 leaves the rest zero
+// N consecutive elements at any alignment of their type (the hardware's global
+// loads take it), in loads of 16 bytes, or one of 8
+typedef u32x4 __attribute__((aligned(2))) any_u32x4;
+typedef unsigned long long __attribute__((aligned(2))) any_u64;
+
+template <typename S, int N>
+__device__ __forceinline__ RawN<S, N> load_n(const S* p) {
+  RawN<S, N> r;
+  if constexpr (sizeof(r) == 8) {
+    __builtin_memcpy(&r, reinterpret_cast<const any_u64*>(p), 8);
+  } else {
+    const any_u32x4* q = reinterpret_cast<const any_u32x4*>(p);
+    u32x4* o = reinterpret_cast<u32x4*>(&r);
+#pragma unroll
+    for (int b = 0; b < static_cast<int>(sizeof(r) / 16); ++b) o[b] = q[b];
+  }
+  return r;
+}
+
+// the first `valid` of them, the rest zero
+template <typename S, int N>
+__device__ __forceinline__ RawN<S, N> load_n(const S* p, int valid) {
+  if (valid >= N) return load_n<S, N>(p);
+  RawN<S, N> r;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r.v[e] = e < valid ? p[e] : static_cast<S>(0.f);
+  return r;
+}
+
 template <typename S>
 __device__ __forceinline__ Raw8<S> load8(const S* p) {
-  typedef u32x4 __attribute__((aligned(2))) any_u32x4;
-  Raw8<S> r;
-  const any_u32x4* q = reinterpret_cast<const any_u32x4*>(p);
-  u32x4* o = reinterpret_cast<u32x4*>(&r);
-  o[0] = q[0];
-  if constexpr (sizeof(S) == 4) o[1] = q[1];
-  return r;
+  return load_n<S, 8>(p);
+}
+template <typename S>
+__device__ __forceinline__ Raw8<S> load8(const S* p, int valid) {
+  return load_n<S, 8>(p, valid);
+}
+template <typename S>
+__device__ __forceinline__ Raw4<S> load4(const S* p, int valid) {
+  return load_n<S, 4>(p, valid);
 }
 
 template <typename S>
-__device__ __forceinline__ Raw8<S> load8(const S* p, int64_t valid) {
-  if (valid >= 8) return load8(p);
-  Raw8<S> r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r.v[e] = e < valid ? p[e] : static_cast<S>(0.f);
-  return r;
-}
-
-template <typename S>
-__device__ __forceinline__ Raw8<S> load8_strided(const S* p, int64_t stride, int64_t valid) {
+__device__ __forceinline__ Raw8<S> load8_strided(const S* p, int64_t stride, int valid) {
   Raw8<S> r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r.v[e] = e < valid ? p[e * stride] : static_cast<S>(0.f);
   return r;
 }
 
-template <typename S>
-__device__ __forceinline__ void store8(S* p, const Raw8<S>& r, int64_t valid) {
-  typedef u32x4 __attribute__((aligned(2))) any_u32x4;
-  if (valid >= 8) {
-    any_u32x4* q = reinterpret_cast<any_u32x4*>(p);
-    const u32x4* o = reinterpret_cast<const u32x4*>(&r);
-    q[0] = o[0];
-    if constexpr (sizeof(S) == 4) q[1] = o[1];
+template <typename S, int N>
+__device__ __forceinline__ void store_n(S* p, const RawN<S, N>& r, int valid) {
+  if (valid >= N) {
+    if constexpr (sizeof(r) == 8) {
+      __builtin_memcpy(reinterpret_cast<any_u64*>(p), &r, 8);
+    } else {
+      any_u32x4* q = reinterpret_cast<any_u32x4*>(p);
+      const u32x4* o = reinterpret_cast<const u32x4*>(&r);
+#pragma unroll
+      for (int b = 0; b < static_cast<int>(sizeof(r) / 16); ++b) q[b] = o[b];
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < N; ++e)
       if (e < valid) p[e] = r.v[e];
   }
 }
@@ -117,6 +144,35 @@ __device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
   for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r.v[e]);
   return f;
 }
+
+// A fragment in LDS: its 16-byte pieces in planes of their own
+template <int N>
+__device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Terms<N>& f) {
+#pragma unroll
+  for (int p = 0; p < N; ++p) lds[p * plane + at] = __builtin_bit_cast(u32x4, f.t[p]);
+}
+__device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Raw8<float>& f) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    u32x4 v;
+    __builtin_memcpy(&v, f.v + 4 * p, 16);
+    lds[p * plane + at] = v;
+  }
+}
+template <int N>
+__device__ __forceinline__ void get_frag(Terms<N>& f, const u32x4* lds, int plane, int at) {
+#pragma unroll
+  for (int p = 0; p < N; ++p) f.t[p] = __builtin_bit_cast(bf16x8, lds[p * plane + at]);
+}
+__device__ __forceinline__ void get_frag(Raw8<float>& f, const u32x4* lds, int plane, int at) {
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const u32x4 v = lds[p * plane + at];
+    __builtin_memcpy(f.v + 4 * p, &v, 16);
+  }
+}
+template <typename F>
+constexpr int kPlanes = sizeof(F) / 16;
 
 template <int N, int M>
 __device__ __forceinline__ void mma(f32x4& acc, const Terms<N>& a, const Terms<M>& b) {
@@ -158,25 +214,57 @@ __device__ __forceinline__ int seg_start(const Segs& sg, int i) {
 
 template <int TT>
 __device__ __forceinline__ Tile find_tile(const Segs& sg, int tile) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, len = sg.nseg + 2;
-  while (len > 1) {                          // 64 candidates at a time
-    const int step = (len + 63) >> 6, i = lane * step;
-    const bool at = i < len && seg_start(sg, lo + i) / TT + lo + i <= tile;
-    const int hits = max(__popcll(__ballot(at)), 1);
-    const int skip = (hits - 1) * step;
-    lo += skip;
-    len = min(step, len - skip);
+  const int lane = threadIdx.x & 63, count = sg.nseg + 2;
+  int lo, first, end, slot;
+  if (count <= 256) {
+    // every start and slot in one round of loads: the search costs one trip to memory
+    int st[4], sl[4], hits = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = q * 64 + lane;
+      st[q] = i < count ? seg_start(sg, i) : static_cast<int>(sg.tokens);
+      sl[q] = i >= 1 && i <= sg.nseg ? sg.slots[i - 1] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = q * 64 + lane;
+      hits += __popcll(__ballot(i < count && st[q] / TT + i <= tile));
+    }
+    lo = max(hits, 1) - 1;
+    first = end = static_cast<int>(sg.tokens);
+    slot = -1;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (lo >> 6 == q) {
+        first = __builtin_amdgcn_readlane(st[q], lo & 63);
+        slot = __builtin_amdgcn_readlane(sl[q], lo & 63);
+      }
+      if ((lo + 1) >> 6 == q) end = __builtin_amdgcn_readlane(st[q], (lo + 1) & 63);
+    }
+  } else {
+    lo = 0;
+    for (int len = count; len > 1;) {        // 64 candidates at a time
+      const int step = (len + 63) >> 6, i = lane * step;
+      const bool at = i < len && seg_start(sg, lo + i) / TT + lo + i <= tile;
+      const int skip = (max(__popcll(__ballot(at)), 1) - 1) * step;
+      lo += skip;
+      len = min(step, len - skip);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    first = seg_start(sg, lo);
+    end = seg_start(sg, lo + 1);
+    slot = lo >= 1 && lo <= sg.nseg ? sg.slots[lo - 1] : -1;
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  const int first = seg_start(sg, lo);
   // numbers that no tile has end here, and so do offsets that do not ascend
   const int64_t t0 = first + static_cast<int64_t>(tile - first / TT - lo) * TT;
-  const int64_t left = seg_start(sg, lo + 1) - t0;
   Tile t;
   t.t0 = static_cast<int>(t0);
-  t.n = t0 < first ? 0 : static_cast<int>(max(int64_t{0}, min(left, int64_t{TT})));
-  t.slot = lo == 0 || lo == sg.nseg + 1 || t.n <= 0 ? -1 : checked_slot(sg.slots, lo - 1, sg.nslots);
+  t.n = t0 < first ? 0 : static_cast<int>(max(int64_t{0}, min(end - t0, int64_t{TT})));
+  t.slot = slot;
+  if (t.n > 0 && (slot < -1 || slot >= sg.nslots)) {
+    count_row_fault();
+    t.slot = -1;
+  }
   return t;
 }
 
@@ -186,254 +274,382 @@ static int tile_count(const Segs& sg) {
 }
 
 // ---------------------------------------------------------------------------
-// shrink: H[t, i] = sum_j W[i, j] x[t, j].  A workgroup of 16 waves takes a tile
-// of 16 NT tokens and one of gridDim.y parts of the width; a wave takes one rank
-// tile and every (16 / rank tiles)-th stretch of 32, and the waves' sums meet in
-// LDS.  W is stored [i][j] (AT false) or [j][i] (AT true).
+// Staging.  A load straight into an operand's lanes would take 16 bytes of 16
+// rows at a time: every 16 bytes a cache line of its own.  So operands that more
+// than one lane group shares, or whose rows are memory's rows, are read in
+// whole lines, brought into fragments once a workgroup, and put into LDS as
+// pieces (row, c) of 8 inner values, piece c at c * (ROWS + 1) + row: 16 rows of
+// a fragment read, and the neighbours that write, fall into different banks.
+//
+// TR false: element (row, inner) at src[row * ld + inner].  TR true: at
+// src[inner * ld + row]; a thread then loads 4 rows of 8 inner values and turns
+// them in registers.  fetch and put are apart so that the next stage's loads are
+// in flight behind this one's products.
 // ---------------------------------------------------------------------------
-constexpr int kShrinkWaves = 16;
+constexpr int kThreads = 256;
 
-template <typename T, typename W, int NT, bool AT>
-__global__ void __launch_bounds__(kShrinkWaves * 64)
+template <typename T, typename S, int ROWS, int PIECES, bool TR>
+struct Stage {
+  using F = Frag<T, S>;
+  static constexpr int kPlane = PIECES * (ROWS + 1);
+  static constexpr int kBytes = kPlane * kPlanes<F> * 16;
+  static constexpr int kUnits = TR ? ROWS / 4 * PIECES : ROWS * PIECES;
+  static constexpr int kEach = (kUnits + kThreads - 1) / kThreads;
+  union Unit {
+    Raw8<S> line;
+    Raw4<S> turn[TR ? 8 : 1];
+  };
+  Unit r[kEach];
+
+  // Inner values from ninner on are zero; rows from nrows on repeat a valid one
+  // (their products are never stored).  Whole pieces take loads without a branch,
+  // all of them in flight at once: a guarded load waits for the one before it.
+  __device__ __forceinline__ void fetch(const S* src, int64_t ld, int nrows, int ninner) {
+    if constexpr (TR) {
+      if (nrows >= ROWS || (nrows >= 4 && nrows % 4 == 0)) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const int u = unit(q), row = min(u % (ROWS / 4) * 4, nrows - 4), k = u / (ROWS / 4) * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            r[q].turn[e] = load_n<S, 4>(src + min(k + e, ninner - 1) * ld + row);
+            if (k + e >= ninner) r[q].turn[e] = Raw4<S>{};
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const int u = unit(q), row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            r[q].turn[e] = load4(src + (k + e) * ld + row, k + e < ninner ? nrows - row : 0);
+        }
+      }
+    } else {
+      if (ninner >= 8 * PIECES || (ninner >= 8 && ninner % 8 == 0)) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const int u = unit(q), k = u % PIECES * 8, row = min(u / PIECES, nrows - 1);
+          r[q].line = load8(src + row * ld + min(k, ninner - 8));
+          if (k >= ninner) r[q].line = Raw8<S>{};
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          const int u = unit(q), k = u % PIECES * 8, row = min(u / PIECES, nrows - 1);
+          r[q].line = load8(src + row * ld + k, ninner - k);
+        }
+      }
+    }
+  }
+
+  // threads beyond the units load the last one again and put nothing
+  static __device__ __forceinline__ int unit(int q) {
+    return min(q * kThreads + static_cast<int>(threadIdx.x), kUnits - 1);
+  }
+
+  __device__ __forceinline__ void put(u32x4* lds) const {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const int u = q * kThreads + static_cast<int>(threadIdx.x);
+      if (kUnits % kThreads != 0 && u >= kUnits) continue;
+      if constexpr (TR) {
+        const int row = u % (ROWS / 4) * 4, c = u / (ROWS / 4);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          F f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r[q].turn[e].v[a]);
+          put_frag(lds, kPlane, c * (ROWS + 1) + row + a, f);
+        }
+      } else {
+        put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, frag_of<T, S>(r[q].line));
+      }
+    }
+  }
+
+  static __device__ __forceinline__ F get(const u32x4* lds, int row, int c) {
+    F f;
+    get_frag(f, lds, kPlane, c * (ROWS + 1) + row);
+    return f;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// shrink: H[t, i] = sum_j W[i, j] x[t, j].  A workgroup takes a tile of 16 NT
+// tokens and one of `parts` parts of the width, a stage of KB columns at a time.
+// NT 4: a wave a token group, all of them on the one staged weight.  NT 1 (short
+// segments, where the weight is the traffic): the waves share the stage's columns
+// and their sums meet in LDS in a fixed order.  W is [i][j] (AT false) or [j][i].
+// ---------------------------------------------------------------------------
+template <typename T, int RT, int NT>
+constexpr int kShrinkCols = NT == 1 ? 512 / RT : (RT == 4 || kPlanes<Frag<T, T>> == 2) ? 128 : 256;
+
+template <typename T, typename W, int RT, int NT, bool AT>
+__global__ void __launch_bounds__(kThreads)
     shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, Segs sg, int width,
-                  int part, int rank, float* __restrict__ H) {
-  __shared__ f32x4 sums[kShrinkWaves][NT][64];
-  const Tile tl = find_tile<16 * NT>(sg, blockIdx.x);
+                  int parts, int part, int rank, float* __restrict__ H) {
+  constexpr int KB = kShrinkCols<T, RT, NT>, PIECES = KB / 8;
+  using SX = Stage<T, T, 16 * NT, PIECES, false>;
+  using SW = Stage<T, W, 16 * RT, PIECES, AT>;
+  __shared__ u32x4 lds[(SX::kBytes + SW::kBytes) / 16];
+  u32x4* const ldw_ = lds + SX::kBytes / 16;
+  const int tile = static_cast<int>(blockIdx.x) / parts, pt = static_cast<int>(blockIdx.x) % parts;
+  const Tile tl = find_tile<16 * NT>(sg, tile);
   if (tl.n <= 0) return;
-  float* Hp = H + (static_cast<int64_t>(blockIdx.y) * sg.tokens + tl.t0) * rank;
+  float* Hp = H + (static_cast<int64_t>(pt) * sg.tokens + tl.t0) * rank;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   if (tl.slot < 0) {
-    for (int i = threadIdx.x; i < tl.n * rank; i += kShrinkWaves * 64) Hp[i] = 0.f;
+    for (int i = threadIdx.x; i < tl.n * rank; i += kThreads) Hp[i] = 0.f;
     return;
   }
-  const int rtiles = (rank + 15) >> 4, parts = kShrinkWaves / rtiles;
-  const int rt = wave % rtiles, kp = wave / rtiles;
-  f32x4 acc[NT] = {};
-  if (kp < parts) {
-    const int j0 = static_cast<int>(blockIdx.y) * part, j1 = min(width, j0 + part);
-    const int i = min(rt * 16 + n, rank - 1);            // rows beyond the rank are not stored
-    const W* wp = w + tl.slot * ldw + (AT ? static_cast<int64_t>(i) : static_cast<int64_t>(i) * width);
-    const T* xp[NT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) xp[u] = x + (tl.t0 + min(u * 16 + n, tl.n - 1)) * ldx;
-    const int full = (j1 - j0) / 32;
-#pragma unroll 4
-    for (int b = kp; b < full; b += parts) {
-      const int j = j0 + b * 32 + g * 8;
-      const Frag<T, W> fw = AT ? frag_of<T, W>(load8_strided(wp + static_cast<int64_t>(j) * rank, rank, 8))
-                               : frag_of<T, W>(load8(wp + j));
-#pragma unroll
-      for (int u = 0; u < NT; ++u) mma(acc[u], fw, frag_of<T, T>(load8(xp[u] + j)));
+  const int j0 = pt * part, j1 = min(width, j0 + part);
+  const T* xs = x + static_cast<int64_t>(tl.t0) * ldx;
+  const W* ws = w + tl.slot * ldw;
+  const int64_t wld = AT ? rank : width;
+  f32x4 acc[RT] = {};
+  SX sx;
+  SW sw;
+  if (j0 < j1) {
+    sx.fetch(xs + j0, ldx, tl.n, j1 - j0);
+    sw.fetch(ws + (AT ? static_cast<int64_t>(j0) * rank : j0), wld, rank, j1 - j0);
+  }
+  for (int j = j0; j < j1; j += KB) {
+    __syncthreads();
+    sx.put(lds);
+    sw.put(ldw_);
+    __syncthreads();
+    if (j + KB < j1) {
+      sx.fetch(xs + j + KB, ldx, tl.n, j1 - j - KB);
+      sw.fetch(ws + (AT ? static_cast<int64_t>(j + KB) * rank : j + KB), wld, rank, j1 - j - KB);
     }
-    if (j0 + full * 32 < j1 && kp == full % parts) {
-      const int j = j0 + full * 32 + g * 8, valid = max(0, min(8, j1 - j));
-      const Frag<T, W> fw = AT ? frag_of<T, W>(load8_strided(wp + static_cast<int64_t>(j) * rank, rank, valid))
-                               : frag_of<T, W>(load8(wp + j, valid));
 #pragma unroll
-      for (int u = 0; u < NT; ++u) mma(acc[u], fw, frag_of<T, T>(load8(xp[u] + j, valid)));
+    for (int b = NT == 1 ? wave : 0; b < KB / 32; b += NT == 1 ? 4 : 1) {
+      const auto fx = SX::get(lds, (NT == 1 ? 0 : wave * 16) + n, b * 4 + g);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) mma(acc[r], SW::get(ldw_, r * 16 + n, b * 4 + g), fx);
     }
   }
+  if constexpr (NT == 1) {
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);
+    __syncthreads();
 #pragma unroll
-  for (int u = 0; u < NT; ++u) sums[wave][u][lane] = acc[u];
-  __syncthreads();
-  for (int q = wave; q < rtiles * NT; q += kShrinkWaves) {
-    const int r = q % rtiles, u = q / rtiles;
-    f32x4 a = sums[r][u][lane];
-    for (int p = 1; p < parts; ++p) a += sums[p * rtiles + r][u][lane];
-    const int t = u * 16 + n, i = r * 16 + g * 4;
-    if (t < tl.n) {
+    for (int r = 0; r < RT; ++r) sums[(wave * RT + r) * 64 + lane] = acc[r];
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < rank) Hp[static_cast<int64_t>(t) * rank + i + e] = a[e];
-    }
+    for (int r = 0; r < RT; ++r)
+      for (int q = 1; q < 4; ++q) acc[r] += sums[(q * RT + r) * 64 + lane];
+  }
+  const int t = (NT == 1 ? 0 : wave * 16) + n;
+  if (t >= tl.n) return;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int i = r * 16 + g * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < rank) Hp[static_cast<int64_t>(t) * rank + i + e] = acc[r][e];
   }
 }
 
 // ---------------------------------------------------------------------------
-// expand: out[t, j] = base[t, j] + scale * sum_i W[i, j] H[t, i].  A wave takes
-// a tile of 16 NT tokens and, step by step, 128 columns.  W is stored [j][i]
-// (AT true) or [i][j] (AT false).  The product's rows are columns of out,
-// permuted so that a lane holds runs of 8 consecutive ones of its token.
-// H comes in `parts` partial sums; the first column block also writes their sum
-// to Hsum when that is asked.
+// expand: out[t, j] = base[t, j] + scale * sum_i W[i, j] H[t, i].  The products'
+// rows are tokens and their columns n * PC + a of out, so a lane holds PC
+// consecutive values of each of its 4 tokens and 16 lanes a stretch of a row.
+// NT 4: a wave a token group, 128 columns of the weight staged for all of them
+// (PC 8).  NT 1: a wave 64 of the 256 staged columns (PC 4).  W is [j][i] (AT true) or [i][j].
+// Neighbouring workgroups take the column blocks of one tile: between them they
+// read whole rows, not the same columns of many.  H comes in `parts` partial
+// sums; the first column block also writes their sum to Hsum when that is asked.
 // ---------------------------------------------------------------------------
-constexpr int kExpandCols = 128;
+template <int NT>
+constexpr int kExpandCols = NT == 1 ? 256 : 128;
 
 template <typename T, typename W, int RK, int NT, bool AT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
     expand_kernel(const T* base, int64_t ldb, const float* __restrict__ H, int parts, const W* __restrict__ w,
-                  int64_t ldw, Segs sg, int width, int span, int rank, float scale, T* out, int64_t ldo,
+                  int64_t ldw, Segs sg, int width, int blocks, int span, int rank, float scale, T* out, int64_t ldo,
                   float* __restrict__ Hsum) {
-  const Tile tl = find_tile<16 * NT>(sg, blockIdx.x);
+  constexpr int COLS = kExpandCols<NT>, PC = NT == 1 ? 4 : 8;
+  using SW = Stage<T, W, COLS, RK * 4, !AT>;
+  __shared__ u32x4 lds[SW::kBytes / 16];
+  const int tile = static_cast<int>(blockIdx.x) / blocks, block = static_cast<int>(blockIdx.x) % blocks;
+  const Tile tl = find_tile<16 * NT>(sg, tile);
   if (tl.n <= 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
-  const int c0 = static_cast<int>(blockIdx.y) * span, c1 = min(width, c0 + span);
+  const int c0 = block * span, c1 = min(width, c0 + span);
   if (tl.slot < 0) {
-    if (Hsum != nullptr && blockIdx.y == 0)
-      for (int i = threadIdx.x; i < tl.n * rank; i += 256) Hsum[static_cast<int64_t>(tl.t0) * rank + i] = 0.f;
+    if (Hsum != nullptr && block == 0)
+      for (int i = threadIdx.x; i < tl.n * rank; i += kThreads) Hsum[static_cast<int64_t>(tl.t0) * rank + i] = 0.f;
     if (base == out) return;
     for (int t = wave; t < tl.n; t += 4)
       for (int j = c0 + lane * 8; j < c1; j += 512) {
         const int valid = min(8, c1 - j);
         Raw8<T> r = {};
         if (base != nullptr) r = load8(base + (tl.t0 + t) * ldb + j, valid);
-        store8(out + (tl.t0 + t) * ldo + j, r, valid);
+        store_n(out + (tl.t0 + t) * ldo + j, r, valid);
       }
     return;
   }
-  Frag<T, float> fh[NT][RK];
+  const W* ws = w + tl.slot * ldw;
+  const int64_t wld = AT ? rank : width;
+  SW sw;
+  sw.fetch(ws + (AT ? static_cast<int64_t>(c0) * rank : c0), wld, width - c0, rank);
+  const int tok = NT == 1 ? 0 : wave * 16;               // the wave's first token
+  Frag<T, float> fh[RK];
 #pragma unroll
-  for (int u = 0; u < NT; ++u)
+  for (int b = 0; b < RK; ++b) {
+    const int t = tok + n, i = b * 32 + g * 8;
+    Raw8<float> h = {};
+    if (t < tl.n) {
+      const int64_t at = static_cast<int64_t>(tl.t0 + t) * rank + i;
+      for (int p = 0; p < parts; ++p) {
+        const Raw8<float> q = load8(H + p * sg.tokens * rank + at, rank - i);
 #pragma unroll
-    for (int b = 0; b < RK; ++b) {
-      const int t = u * 16 + n, i = b * 32 + g * 8;
-      Raw8<float> h = {};
-      if (t < tl.n) {
-        const int64_t at = static_cast<int64_t>(tl.t0 + t) * rank + i;
-        for (int p = 0; p < parts; ++p) {
-          const Raw8<float> q = load8(H + p * sg.tokens * rank + at, rank - i);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h.v[e] += q.v[e];
-        }
-        if (Hsum != nullptr && blockIdx.y == 0 && wave == 0) store8(Hsum + at, h, rank - i);
+        for (int e = 0; e < 8; ++e) h.v[e] += q.v[e];
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h.v[e] *= scale;
-      fh[u][b] = frag_of<T, float>(h);
+      if (Hsum != nullptr && block == 0 && (NT == 4 || wave == 0)) store_n(Hsum + at, h, rank - i);
     }
-  const W* wc = w + tl.slot * ldw;
-  for (int j0 = c0 + wave * kExpandCols; j0 < c1; j0 += 4 * kExpandCols) {
-    f32x4 acc[NT][8] = {};
 #pragma unroll
-    for (int b = 0; b < RK; ++b) {
-      const int i = b * 32 + g * 8;
-      if constexpr (AT) {
-        // row q of product a is column j0 + (a / 2) * 32 + (q / 4) * 8 + (a % 2) * 4 + q % 4
+    for (int e = 0; e < 8; ++e) h.v[e] *= scale;
+    fh[b] = frag_of<T, float>(h);
+  }
+  for (int j0 = c0; j0 < c1; j0 += COLS) {
+    const int row = (NT == 1 ? wave * 64 : 0) + n * PC, j = j0 + row;    // this lane's columns
+    RawN<T, PC> r[4] = {};
+    if (base != nullptr) {
+      const T* bp[4];
 #pragma unroll
-        for (int a = 0; a < 8; ++a) {
-          const int j = min(j0 + (a >> 1) * 32 + (n >> 2) * 8 + (a & 1) * 4 + (n & 3), width - 1);
-          const Frag<T, W> fw = frag_of<T, W>(load8(wc + static_cast<int64_t>(j) * rank + i, rank - i));
+      for (int q = 0; q < 4; ++q) bp[q] = base + (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j;
+      if (j0 + COLS <= c1) {
 #pragma unroll
-          for (int u = 0; u < NT; ++u) mma(acc[u][a], fw, fh[u][b]);
-        }
+        for (int q = 0; q < 4; ++q) r[q] = load_n<T, PC>(bp[q]);
       } else {
-        // row q of product a is column j0 + q * 8 + a: 8 loads of 8 columns hold 8 products' operands
-        Frag<T, W> fw[8];
-        const int j = j0 + n * 8, valid = max(0, min(8, width - j));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const Raw8<W> r = load8(wc + static_cast<int64_t>(i + e) * width + j, i + e < rank ? valid : 0);
-#pragma unroll
-          for (int a = 0; a < 8; ++a) put_elem<T, W>(fw[a], e, r.v[a]);
-        }
-#pragma unroll
-        for (int a = 0; a < 8; ++a)
-#pragma unroll
-          for (int u = 0; u < NT; ++u) mma(acc[u][a], fw[a], fh[u][b]);
+        for (int q = 0; q < 4; ++q) r[q] = load_n<T, PC>(bp[q], c1 - j);
       }
     }
+    __syncthreads();
+    sw.put(lds);
+    __syncthreads();
+    if (j0 + COLS < c1)
+      sw.fetch(ws + (AT ? static_cast<int64_t>(j0 + COLS) * rank : j0 + COLS), wld, width - j0 - COLS, rank);
+    f32x4 acc[PC] = {};
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int t = u * 16 + n;
+    for (int b = 0; b < RK; ++b)
+#pragma unroll
+      for (int a = 0; a < PC; ++a) mma(acc[a], fh[b], SW::get(lds, row + a, b * 4 + g));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int t = tok + g * 4 + q;
       if (t >= tl.n) continue;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int j = AT ? j0 + q * 32 + g * 8 : j0 + (g * 4 + q) * 8;
-        const int valid = min(8, c1 - j);
-        if (valid <= 0) continue;
-        Raw8<T> r = {};
-        if (base != nullptr) r = load8(base + (tl.t0 + t) * ldb + j, valid);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          r.v[e] = from_f32<T>(to_f32(r.v[e]) + (AT ? acc[u][2 * q + (e >> 2)][e & 3] : acc[u][e][q]));
-        store8(out + (tl.t0 + t) * ldo + j, r, valid);
-      }
+      for (int a = 0; a < PC; ++a) r[q].v[a] = from_f32<T>(to_f32(r[q].v[a]) + acc[a][q]);
+      store_n(out + (tl.t0 + t) * ldo + j, r[q], j0 + COLS <= c1 ? PC : c1 - j);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 // outer: G_c[i, j] = scale * sum over the tokens t of slot c of H[t, i] x[t, j].
-// A workgroup takes one slot, 128 columns and every gridDim.z-th group of 32 of
-// its tokens, the 4 waves in turn.  The inner index is the token: a lane loads
-// 8 columns of each of its 8 tokens, which are the operands of 8 products with
-// columns n * 8 + a.  With one part the sums go to G ([i][j], or [j][i] with AT),
-// else each part's to its own copy (slot stride rank * width) for join_parts.
+// The inner index is the token.  A workgroup takes one slot, 64 PC columns and
+// every gridDim.z-th stage of 128 of its tokens; H is staged for the 4 waves,
+// which own 16 PC columns each: a lane loads PC columns of 8 tokens, the
+// operands of PC products with columns n * PC + a.  With one part the sums go to
+// G ([i][j], or [j][i] with AT), else each part's to its own copy (slot stride
+// rank * width) for join_parts.
 // ---------------------------------------------------------------------------
-constexpr int kOuterCols = 128;
+constexpr int kOuterTokens = 128;
 
-template <typename T, int RT, bool AT>
-__global__ void __launch_bounds__(256)
+template <typename T, int RT, int PC, bool AT>
+__global__ void __launch_bounds__(kThreads)
     outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
                  float scale, float* __restrict__ G, int64_t ldg, int64_t part_stride, int accumulate) {
-  __shared__ f32x4 sums[2][RT * 8][64];
+  using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true>;
+  __shared__ u32x4 lds[SH::kBytes / 16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
-  const int c = blockIdx.y, j = static_cast<int>(blockIdx.x) * kOuterCols + n * 8;
-  const int valid = max(0, min(8, width - j));
-  const int turns = 4 * static_cast<int>(gridDim.z), mine = static_cast<int>(blockIdx.z) * 4 + wave;
-  f32x4 acc[RT][8] = {};
-  int group = 0;
+  const int c = blockIdx.y, j = ((static_cast<int>(blockIdx.x) * 4 + wave) * 16 + n) * PC;
+  const int valid = max(0, min(PC, width - j));
+  const bool whole = (static_cast<int>(blockIdx.x) + 1) * 64 * PC <= width;
+  const int turns = static_cast<int>(gridDim.z);
+  f32x4 acc[RT][PC] = {};
+  int turn = static_cast<int>(blockIdx.z);                 // stages until this part's next
   bool any = false;
   for (int s0 = 0; s0 < sg.nseg; s0 += 64) {
     unsigned long long hits = __ballot(s0 + lane < sg.nseg && sg.slots[min(s0 + lane, sg.nseg - 1)] == c);
     for (; hits != 0; hits &= hits - 1) {
       const int s = s0 + __ffsll(hits) - 1;
       const int t0 = seg_start(sg, s + 1), t1 = seg_start(sg, s + 2);
-      any |= t1 > t0;
-      for (int t = t0; t < t1; t += 32, ++group) {
-        if (group % turns != mine) continue;
-        const int tg = t + g * 8, left = t1 - tg;          // tokens of other segments enter as zeros
-        Frag<T, T> fx[8];
-        Frag<T, float> fh[RT];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const Raw8<T> r = load8(x + static_cast<int64_t>(min(tg + e, t1 - 1)) * ldx + j, e < left ? valid : 0);
-#pragma unroll
-          for (int a = 0; a < 8; ++a) put_elem<T, T>(fx[a], e, r.v[a]);
+      if (t1 <= t0) continue;
+      any = true;
+      for (int t = t0; t < t1; t += kOuterTokens) {
+        if (turn != 0) {
+          --turn;
+          continue;
         }
+        turn = turns - 1;
+        const int left = min(kOuterTokens, t1 - t);
+        SH sh;
+        sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left);
+        RawN<T, PC> cur[8], nxt[8];
+        auto fetch = [&](RawN<T, PC>(&q)[8], int b) {         // tokens of other segments enter as zeros
+          if (whole) {
 #pragma unroll
-        for (int b = 0; b < RT; ++b) {
-          const int i = b * 16 + n;
-          fh[b] = frag_of<T, float>(load8_strided(H + static_cast<int64_t>(tg) * rank + i, rank, i < rank ? left : 0));
+            for (int e = 0; e < 8; ++e) {
+              const int k = b * 32 + g * 8 + e;
+              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j);
+              if (k >= left) q[e] = RawN<T, PC>{};
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int k = b * 32 + g * 8 + e;
+              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j, k < left ? valid : 0);
+            }
+          }
+        };
+        fetch(cur, 0);
+        __syncthreads();
+        sh.put(lds);
+        __syncthreads();
+        for (int b = 0; b * 32 < left; ++b) {
+          if (b * 32 + 32 < left) fetch(nxt, b + 1);
+          Frag<T, T> fx[PC];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, cur[e].v[a]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);
+#pragma unroll
+            for (int a = 0; a < PC; ++a) mma(acc[r][a], fh, fx[a]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) cur[e] = nxt[e];
         }
-#pragma unroll
-        for (int b = 0; b < RT; ++b)
-#pragma unroll
-          for (int a = 0; a < 8; ++a) mma(acc[b][a], fh[b], fx[a]);
       }
     }
   }
-  // the waves' sums in a fixed order: (0 + 2) + (1 + 3)
-#pragma unroll
-  for (int half = 2; half >= 1; half >>= 1) {
-    __syncthreads();
-    if (wave >= half && wave < 2 * half)
-#pragma unroll
-      for (int q = 0; q < RT * 8; ++q) sums[wave - half][q][lane] = acc[q >> 3][q & 7];
-    __syncthreads();
-    if (wave < half)
-#pragma unroll
-      for (int q = 0; q < RT * 8; ++q) acc[q >> 3][q & 7] += sums[wave][q][lane];
-  }
-  if (wave != 0 || (accumulate && !any && gridDim.z == 1)) return;
   const bool last = gridDim.z == 1;
+  if (last && accumulate && !any) return;
   const bool add = last && accumulate;
   float* gc = G + blockIdx.z * part_stride + c * ldg;
   const float f = last ? scale : 1.f;
 #pragma unroll
-  for (int b = 0; b < RT; ++b)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int i = b * 16 + g * 4 + q;
+      const int i = r * 16 + g * 4 + q;
       if (i >= rank) continue;
 #pragma unroll
-      for (int a = 0; a < 8; ++a) {
+      for (int a = 0; a < PC; ++a) {
         if (a >= valid) continue;
         float* p = gc + (AT && last ? static_cast<int64_t>(j + a) * rank + i : static_cast<int64_t>(i) * width + j + a);
-        const float v = f * acc[b][a][q];
+        const float v = f * acc[r][a][q];
         *p = add ? *p + v : v;
       }
     }
@@ -493,25 +709,26 @@ static int check_common(const Segs& sg, const Shape& sh, const void* x, int64_t 
 // ---------------------------------------------------------------------------
 constexpr int kMaxParts = 16;
 
-// Parts of the width that shrink sums apart.  A tile's workgroup reads a whole
-// client's weight, so with fewer tiles than compute units the width is split
-// until there are enough workgroups, a part never below 512 columns.
-static int shrink_parts(int64_t tokens, int64_t width) {
+// Token groups of 16 a tile: 4 where segments are long enough to fill most of
+// them, else 1.
+static int tile_groups(int64_t tokens, int nseg) { return tokens >= 32 * static_cast<int64_t>(nseg) ? 4 : 1; }
+
+// Parts of the width that shrink sums apart: two workgroups a compute unit where
+// the tiles alone give fewer, a part never below 512 columns.
+static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
+  const int64_t tiles = tokens / (16 * tile_groups(tokens, nseg)) + std::min<int64_t>(nseg, tokens);
   int p = 1;
-  while (p < kMaxParts && tokens * p < 64 && width >= 1024 * p) p *= 2;
+  while (p < kMaxParts && tiles * p < 512 && width >= 1024 * p) p *= 2;
   return p;
 }
 
-// Tokens per tile / 16: the most that still leaves a workgroup a compute unit.
-static int tile_width(int64_t tokens) { return tokens >= 64 * 256 ? 4 : tokens >= 32 * 256 ? 2 : 1; }
-
-// Parts of a client's tokens that outer sums apart: enough workgroups for the
-// card, each with at least 8 groups of 32 tokens.
-static int outer_parts(int64_t tokens, int64_t width, int nslots) {
-  const int64_t blocks = cdiv(width, kOuterCols) * nslots;
-  const int64_t groups = cdiv(tokens, 32 * static_cast<int64_t>(nslots));
+// Parts of a client's tokens that outer sums apart: two workgroups a compute
+// unit, each with at least 2 stages of tokens.
+static int outer_parts(int64_t tokens, int nslots, int64_t width, int rank) {
+  const int64_t blocks = cdiv(width, rank <= 32 ? 512 : 256) * nslots;
+  const int64_t stages = cdiv(tokens, kOuterTokens * static_cast<int64_t>(nslots));
   int p = 1;
-  while (p < kMaxParts && blocks * p < 512 && groups >= 16 * p) p *= 2;
+  while (p < kMaxParts && blocks * p < 512 && stages >= 4 * p) p *= 2;
   return p;
 }
 
@@ -519,36 +736,39 @@ struct Workspace {
   size_t h, z, ga, gb, bytes;
 };
 
-static Workspace plan(int64_t tokens, int64_t k, int64_t m, int rank, int nslots) {
+static Workspace plan(int64_t tokens, int nseg, int nslots, int64_t k, int64_t m, int rank) {
   const size_t row = static_cast<size_t>(rank) * 4;
-  const int pa = outer_parts(tokens, k, nslots), pb = outer_parts(tokens, m, nslots);
+  const int pa = outer_parts(tokens, nslots, k, rank), pb = outer_parts(tokens, nslots, m, rank);
   Workspace w{};
   w.h = 0;
-  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, k);
-  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, m) + 1);
+  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, nseg, k);
+  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, nseg, m) + 1);
   w.gb = w.ga + (pa > 1 ? static_cast<size_t>(pa) * nslots * k * row : 0);
   w.bytes = w.gb + (pb > 1 ? static_cast<size_t>(pb) * nslots * m * row : 0) + 16;
   return w;
 }
 
+// f(groups, rank tiles) as constants
 template <typename F>
-static int with_tile(int64_t tokens, F&& f) {
-  switch (tile_width(tokens)) {
-    case 4: return f(std::integral_constant<int, 4>{});
-    case 2: return f(std::integral_constant<int, 2>{});
-    default: return f(std::integral_constant<int, 1>{});
-  }
+static int with_tile(const Segs& sg, int rank, F&& f) {
+  auto ranks = [&](auto nt) {
+    if (rank <= 16) return f(nt, std::integral_constant<int, 1>{});
+    if (rank <= 32) return f(nt, std::integral_constant<int, 2>{});
+    return f(nt, std::integral_constant<int, 4>{});
+  };
+  return tile_groups(sg.tokens, sg.nseg) == 4 ? ranks(std::integral_constant<int, 4>{})
+                                              : ranks(std::integral_constant<int, 1>{});
 }
 
 template <typename T, typename W, bool AT>
 static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw, const Segs& sg, int64_t width,
                          int parts, int rank, float* H, hipStream_t st) {
-  const int part = static_cast<int>(cdiv(cdiv(width, parts), 32) * 32);
-  return with_tile(sg.tokens, [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
-    hipLaunchKernelGGL((shrink_kernel<T, W, NT, AT>), dim3(tile_count<16 * NT>(sg), parts), dim3(kShrinkWaves * 64),
-                       0, st, static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, sg,
-                       static_cast<int>(width), part, rank, H);
+  return with_tile(sg, rank, [&](auto nt, auto rt) {
+    constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, KB = kShrinkCols<T, RT, NT>;
+    const int part = static_cast<int>(cdiv(cdiv(width, parts), KB) * KB);
+    hipLaunchKernelGGL((shrink_kernel<T, W, RT, NT, AT>), dim3(tile_count<16 * NT>(sg) * parts), dim3(kThreads), 0, st,
+                       static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, sg, static_cast<int>(width),
+                       parts, part, rank, H);
     return launch_status("shrink_kernel");
   });
 }
@@ -557,39 +777,33 @@ template <typename T, typename W, bool AT>
 static int launch_expand(const void* base, int64_t ldb, const float* H, int parts, const void* w, int64_t ldw,
                          const Segs& sg, int64_t width, int rank, float scale, void* out, int64_t ldo, float* Hsum,
                          hipStream_t st) {
-  return with_tile(sg.tokens, [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
+  return with_tile(sg, rank, [&](auto nt, auto rt) {
+    constexpr int NT = decltype(nt)::value, RK = decltype(rt)::value == 4 ? 2 : 1, COLS = kExpandCols<NT>;
     const int tiles = tile_count<16 * NT>(sg);
-    // at least 2048 workgroups where the width allows it
-    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, tiles), cdiv(width, 4 * kExpandCols)));
-    const int span = static_cast<int>(cdiv(cdiv(width, blocks), 4 * kExpandCols) * 4 * kExpandCols);
-    const dim3 grid(tiles, static_cast<unsigned>(cdiv(width, span)));
-    auto go = [&](auto rk) {
-      constexpr int RK = decltype(rk)::value;
-      hipLaunchKernelGGL((expand_kernel<T, W, RK, NT, AT>), grid, dim3(256), 0, st, static_cast<const T*>(base), ldb,
-                         H, parts, static_cast<const W*>(w), ldw, sg, static_cast<int>(width), span, rank, scale,
-                         static_cast<T*>(out), ldo, Hsum);
-      return launch_status("expand_kernel");
-    };
-    return rank <= 32 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
+    // four workgroups a compute unit where the width allows it
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, tiles), cdiv(width, COLS)));
+    const int span = static_cast<int>(cdiv(cdiv(width, want), COLS) * COLS);
+    const int blocks = static_cast<int>(cdiv(width, span));
+    hipLaunchKernelGGL((expand_kernel<T, W, RK, NT, AT>), dim3(static_cast<unsigned>(tiles) * blocks), dim3(kThreads),
+                       0, st, static_cast<const T*>(base), ldb, H, parts, static_cast<const W*>(w), ldw, sg,
+                       static_cast<int>(width), blocks, span, rank, scale, static_cast<T*>(out), ldo, Hsum);
+    return launch_status("expand_kernel");
   });
 }
 
 template <typename T, bool AT>
 static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& sg, int64_t width, int rank,
                         float scale, float* G, int64_t ldg, int accumulate, float* parts_ws, hipStream_t st) {
-  const int parts = outer_parts(sg.tokens, width, sg.nslots);
+  const int parts = outer_parts(sg.tokens, sg.nslots, width, rank);
   const int64_t per = rank * width, stride = per * sg.nslots;
-  const dim3 grid(static_cast<unsigned>(cdiv(width, kOuterCols)), static_cast<unsigned>(sg.nslots), parts);
-  auto go = [&](auto rt) {
-    constexpr int RT = decltype(rt)::value;
-    hipLaunchKernelGGL((outer_kernel<T, RT, AT>), grid, dim3(256), 0, st, static_cast<const T*>(x), ldx, H, sg,
-                       static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg, stride,
-                       accumulate);
+  const int rc = with_tile(sg, rank, [&](auto, auto rt) {
+    constexpr int RT = decltype(rt)::value, PC = RT == 4 ? 4 : 8;
+    const dim3 grid(static_cast<unsigned>(cdiv(width, 64 * PC)), static_cast<unsigned>(sg.nslots), parts);
+    hipLaunchKernelGGL((outer_kernel<T, RT, PC, AT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx, H,
+                       sg, static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg,
+                       stride, accumulate);
     return launch_status("outer_kernel");
-  };
-  const int rc = rank <= 16 ? go(std::integral_constant<int, 1>{})
-                            : rank <= 32 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
+  });
   if (rc || parts == 1) return rc;
   const dim3 jg(static_cast<unsigned>(cdiv(per, 256)), static_cast<unsigned>(sg.nslots));
   hipLaunchKernelGGL((join_parts_kernel<AT>), jg, dim3(256), 0, st, parts_ws, parts, stride, sg,
@@ -607,7 +821,7 @@ struct Weights {
 template <typename T, typename W>
 static int run_apply(const void* base, int64_t ldbase, const void* x, int64_t ldx, const Weights& w, const Segs& sg,
                      const Shape& sh, void* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
-  const int parts = shrink_parts(sg.tokens, sh.k);
+  const int parts = shrink_parts(sg.tokens, sg.nseg, sh.k);
   float* H = parts == 1 && hidden != nullptr ? hidden : reinterpret_cast<float*>(ws);
   if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, parts, sh.rank, H, st)) return rc;
   return launch_expand<T, W, true>(base, ldbase, H, parts, w.B, w.ldb, sg, sh.m, sh.rank, sh.scale, out, ldo,
@@ -636,7 +850,7 @@ static int run_grad(const void* dout, int64_t lddo, const void* x, int64_t ldx, 
   if (sg.tokens > 0) {
     if (g.dx != nullptr || g.dA != nullptr) {
       // the parts of z meet in the expand that needs them; without one there is one part
-      const int parts = g.dx != nullptr ? shrink_parts(sg.tokens, sh.m) : 1;
+      const int parts = g.dx != nullptr ? shrink_parts(sg.tokens, sg.nseg, sh.m) : 1;
       float* Zp = Z;
       if (parts > 1) Z = Zp + static_cast<int64_t>(parts) * sg.tokens * sh.rank;
       if (int rc = launch_shrink<T, W, true>(dout, lddo, w.B, w.ldb, sg, sh.m, parts, sh.rank, Zp, st)) return rc;
@@ -672,15 +886,17 @@ static int with_types(int32_t dtype, int32_t wdtype, F&& f) {
 
 using namespace sra;
 
-extern "C" int sra_adapter_workspace_bytes(int64_t tokens, int64_t k, int64_t m, int32_t rank, int32_t nslots,
-                                           size_t* bytes) {
+extern "C" int sra_adapter_workspace_bytes(int64_t tokens, int32_t nseg, int32_t nslots, int64_t k, int64_t m,
+                                           int32_t rank, size_t* bytes) {
   SRA_REQUIRE(bytes != nullptr, SRA_ERR_ARG, "null bytes pointer");
   if (int rc = check_tokens(tokens, nslots)) return rc;
-  SRA_REQUIRE(k >= 1 && m >= 1, SRA_ERR_SHAPE, "k and m must be >= 1");
+  SRA_REQUIRE(nseg >= 0, SRA_ERR_ARG, "nseg must be >= 0, got %d", nseg);
+  SRA_REQUIRE(k >= 1 && m >= 1 && k < (int64_t{1} << 31) && m < (int64_t{1} << 31), SRA_ERR_SHAPE,
+              "k and m must be in [1, 2^31), got %lld, %lld", static_cast<long long>(k), static_cast<long long>(m));
   SRA_REQUIRE(rank >= 1, SRA_ERR_ARG, "rank must be >= 1, got %d", rank);
   SRA_REQUIRE(rank <= SRA_ADAPTER_MAX_RANK, SRA_ERR_UNSUPPORTED, "rank %d is above %d", rank,
               SRA_ADAPTER_MAX_RANK);
-  *bytes = plan(tokens, k, m, rank, nslots).bytes;
+  *bytes = plan(tokens, nseg, nslots, k, m, rank).bytes;
   return SRA_OK;
 }
 
@@ -698,7 +914,7 @@ extern "C" int sra_adapter_apply(const void* base, int64_t ldbase, const void* x
   SRA_REQUIRE(base != out || ldbase == ldo || tokens <= 1, SRA_ERR_SHAPE, "base and out are one buffer with two row strides");
   if (tokens == 0) return SRA_OK;
   size_t need = 0;
-  if (int rc = sra_adapter_workspace_bytes(tokens, k, m, rank, nslots, &need)) return rc;
+  if (int rc = sra_adapter_workspace_bytes(tokens, nseg, nslots, k, m, rank, &need)) return rc;
   SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "adapter workspace: need %zu bytes, got %zu", need,
               ws_bytes);
   const Weights wt{A, lda, B, ldb};
@@ -730,13 +946,13 @@ extern "C" int sra_adapter_grad(const void* dout, int64_t lddo, const void* x, i
               "gradients of %d slots: more than 65535", nslots);
   if (dx == nullptr && dA == nullptr && dB == nullptr) return SRA_OK;
   size_t need = 0;
-  if (int rc = sra_adapter_workspace_bytes(tokens, k, m, rank, nslots, &need)) return rc;
+  if (int rc = sra_adapter_workspace_bytes(tokens, nseg, nslots, k, m, rank, &need)) return rc;
   SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "adapter workspace: need %zu bytes, got %zu", need,
               ws_bytes);
   const GradOut g{hidden, dxbase, lddxb, dx, lddx, dA, ldda, dB, lddb, accumulate};
   const Weights wt{A, lda, B, ldb};
   return with_types(dtype, wdtype, [&](auto t, auto w) {
     return run_grad<decltype(t), decltype(w)>(dout, lddo, x, ldx, wt, sg, sh, g, static_cast<char*>(ws),
-                                              plan(tokens, k, m, rank, nslots), static_cast<hipStream_t>(stream));
+                                              plan(tokens, nseg, nslots, k, m, rank), static_cast<hipStream_t>(stream));
   });
 }

@@ -149,8 +149,8 @@ def _adapter_args(x, A, B, offsets, slots):
     return head, keep, T, K, M, n, r, dtype, _DTYPES[A.dtype]
 
 
-def _adapter_workspace(T, K, M, r, n, device):
-    nb = _lib.query_bytes("sra_adapter_workspace_bytes", T, K, M, r, n)
+def _adapter_workspace(T, S, n, K, M, r, device):
+    nb = _lib.query_bytes("sra_adapter_workspace_bytes", T, S, n, K, M, r)
     return engine._workspace(nb, device), nb
 
 
@@ -172,7 +172,7 @@ def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=Fal
         out = torch.empty((T, M), dtype=x.dtype, device=dev)
     out, ldo = _rows("out", out, (T, M), x.dtype, dev, out=True)
     H = torch.empty((T, r), dtype=torch.float32, device=dev) if hidden else None
-    ws, nb = _adapter_workspace(T, K, M, r, n, dev)
+    ws, nb = _adapter_workspace(T, slots.shape[0], n, K, M, r, dev)
     _call(dev, "sra_adapter_apply", _ptr(base), ldbase, *head, float(scale), dtype, wdtype, out.data_ptr(), ldo,
           _ptr(H), ws.data_ptr(), nb)
     return (out, H) if hidden else out
@@ -211,7 +211,7 @@ def adapter_grad(grad_out, x, A, B, offsets, slots, scale=1.0, hidden=None, base
                       lambda a, t: _slot_rows(a, t, (n, r, K), dev, torch.float32, out=True))
     dB, lddb = target("grad_B", grad_B, lambda: torch.empty((n, M, r), dtype=torch.float32, device=dev),
                       lambda a, t: _slot_rows(a, t, (n, M, r), dev, torch.float32, out=True))
-    ws, nb = _adapter_workspace(T, K, M, r, n, dev)
+    ws, nb = _adapter_workspace(T, slots.shape[0], n, K, M, r, dev)
     _call(dev, "sra_adapter_grad", dy.data_ptr(), lddy, *head, float(scale), dtype, wdtype, _ptr(hidden),
           _ptr(base_grad), lddxb, _ptr(dx), lddx, _ptr(dA), ldda, _ptr(dB), lddb, int(bool(accumulate)),
           ws.data_ptr(), nb)

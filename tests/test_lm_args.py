@@ -41,9 +41,9 @@ def test_adapter_apply_refuses(kw, exc, match):
 
 def test_adapter_workspace_refuses():
     with pytest.raises(NotImplementedError):
-        _lib.query_bytes("sra_adapter_workspace_bytes", 8, 64, 64, 65, 1)
+        _lib.query_bytes("sra_adapter_workspace_bytes", 8, 1, 1, 64, 64, 65)
     with pytest.raises(ValueError):
-        _lib.query_bytes("sra_adapter_workspace_bytes", 8, 0, 64, 8, 1)
+        _lib.query_bytes("sra_adapter_workspace_bytes", 8, 1, 1, 0, 64, 8)
 
 
 @pytest.mark.parametrize("kw,exc,match", [

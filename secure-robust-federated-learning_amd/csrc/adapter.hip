@@ -35,9 +35,24 @@ unsigned int adapter_row_faults(bool reset) { return tu_row_faults(reset); }
 // ---------------------------------------------------------------------------
 // 8 values a lane, and their products
 // ---------------------------------------------------------------------------
+// N stored values as they came, in words: a load's registers stay untouched, and
+// unwaited for, until get takes a value out of them.
 template <typename S, int N>
 struct RawN {
-  S v[N];
+  static constexpr int kWords = N * static_cast<int>(sizeof(S)) / 4;
+  unsigned w[kWords];
+  __device__ __forceinline__ S get(int e) const {
+    if constexpr (sizeof(S) == 4) return __builtin_bit_cast(S, w[e]);
+    else return __builtin_bit_cast(S, static_cast<unsigned short>(w[e / 2] >> (e % 2 * 16)));
+  }
+  __device__ __forceinline__ void set(int e, S v) {
+    if constexpr (sizeof(S) == 4) {
+      w[e] = __builtin_bit_cast(unsigned, v);
+    } else {
+      const unsigned b = __builtin_bit_cast(unsigned short, v);
+      w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | b << 16 : (w[e / 2] & 0xffff0000u) | b;
+    }
+  }
 };
 template <typename S>
 using Raw8 = RawN<S, 8>;
@@ -47,18 +62,23 @@ using Raw4 = RawN<S, 4>;
 // N consecutive elements at any alignment of their type (the hardware's global
 // loads take it), in loads of 16 bytes, or one of 8
 typedef u32x4 __attribute__((aligned(2))) any_u32x4;
-typedef unsigned long long __attribute__((aligned(2))) any_u64;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 __attribute__((aligned(2))) any_u32x2;
 
 template <typename S, int N>
 __device__ __forceinline__ RawN<S, N> load_n(const S* p) {
   RawN<S, N> r;
   if constexpr (sizeof(r) == 8) {
-    __builtin_memcpy(&r, reinterpret_cast<const any_u64*>(p), 8);
+    const u32x2 v = *reinterpret_cast<const any_u32x2*>(p);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
   } else {
-    const any_u32x4* q = reinterpret_cast<const any_u32x4*>(p);
-    u32x4* o = reinterpret_cast<u32x4*>(&r);
 #pragma unroll
-    for (int b = 0; b < static_cast<int>(sizeof(r) / 16); ++b) o[b] = q[b];
+    for (int b = 0; b < r.kWords / 4; ++b) {
+      const u32x4 v = reinterpret_cast<const any_u32x4*>(p)[b];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.w[b * 4 + e] = v[e];
+    }
   }
   return r;
 }
@@ -67,9 +87,10 @@ __device__ __forceinline__ RawN<S, N> load_n(const S* p) {
 template <typename S, int N>
 __device__ __forceinline__ RawN<S, N> load_n(const S* p, int valid) {
   if (valid >= N) return load_n<S, N>(p);
-  RawN<S, N> r;
+  RawN<S, N> r = {};
 #pragma unroll
-  for (int e = 0; e < N; ++e) r.v[e] = e < valid ? p[e] : static_cast<S>(0.f);
+  for (int e = 0; e < N; ++e)
+    if (e < valid) r.set(e, p[e]);
   return r;
 }
 
@@ -86,35 +107,29 @@ __device__ __forceinline__ Raw4<S> load4(const S* p, int valid) {
   return load_n<S, 4>(p, valid);
 }
 
-template <typename S>
-__device__ __forceinline__ Raw8<S> load8_strided(const S* p, int64_t stride, int valid) {
-  Raw8<S> r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r.v[e] = e < valid ? p[e * stride] : static_cast<S>(0.f);
-  return r;
-}
-
 template <typename S, int N>
 __device__ __forceinline__ void store_n(S* p, const RawN<S, N>& r, int valid) {
   if (valid >= N) {
     if constexpr (sizeof(r) == 8) {
-      __builtin_memcpy(reinterpret_cast<any_u64*>(p), &r, 8);
+      *reinterpret_cast<any_u32x2*>(p) = u32x2{r.w[0], r.w[1]};
     } else {
-      any_u32x4* q = reinterpret_cast<any_u32x4*>(p);
-      const u32x4* o = reinterpret_cast<const u32x4*>(&r);
 #pragma unroll
-      for (int b = 0; b < static_cast<int>(sizeof(r) / 16); ++b) q[b] = o[b];
+      for (int b = 0; b < r.kWords / 4; ++b)
+        reinterpret_cast<any_u32x4*>(p)[b] = u32x4{r.w[b * 4], r.w[b * 4 + 1], r.w[b * 4 + 2], r.w[b * 4 + 3]};
     }
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (e < valid) p[e] = r.v[e];
+      if (e < valid) p[e] = r.get(e);
   }
 }
 
 template <int N>
 struct Terms {
   bf16x8 t[N];
+};
+struct Floats {
+  float v[8];
 };
 
 // nearest bf16 and the rest
@@ -127,7 +142,7 @@ __device__ __forceinline__ void split_into(Terms<2>& f, int e, float x) {
 
 // the operand that T's matrix units take for stored values S
 template <typename T, typename S>
-using Frag = std::conditional_t<std::is_same_v<T, float>, Raw8<float>,
+using Frag = std::conditional_t<std::is_same_v<T, float>, Floats,
                                 Terms<std::is_same_v<S, __bf16> ? 1 : 2>>;
 
 template <typename T, typename S>
@@ -140,8 +155,12 @@ __device__ __forceinline__ void put_elem(Frag<T, S>& f, int e, S x) {
 template <typename T, typename S>
 __device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
   Frag<T, S> f;
+  if constexpr (std::is_same_v<S, __bf16>) {
+    f.t[0] = __builtin_bit_cast(bf16x8, u32x4{r.w[0], r.w[1], r.w[2], r.w[3]});
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r.v[e]);
+    for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r.get(e));
+  }
   return f;
 }
 
@@ -151,7 +170,7 @@ __device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Te
 #pragma unroll
   for (int p = 0; p < N; ++p) lds[p * plane + at] = __builtin_bit_cast(u32x4, f.t[p]);
 }
-__device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Raw8<float>& f) {
+__device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Floats& f) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     u32x4 v;
@@ -164,7 +183,7 @@ __device__ __forceinline__ void get_frag(Terms<N>& f, const u32x4* lds, int plan
 #pragma unroll
   for (int p = 0; p < N; ++p) f.t[p] = __builtin_bit_cast(bf16x8, lds[p * plane + at]);
 }
-__device__ __forceinline__ void get_frag(Raw8<float>& f, const u32x4* lds, int plane, int at) {
+__device__ __forceinline__ void get_frag(Floats& f, const u32x4* lds, int plane, int at) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const u32x4 v = lds[p * plane + at];
@@ -183,7 +202,7 @@ __device__ __forceinline__ void mma(f32x4& acc, const Terms<N>& a, const Terms<M
       if (i + j < 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t[i], b.t[j], acc, 0, 0, 0);
 }
 
-__device__ __forceinline__ void mma(f32x4& acc, const Raw8<float>& a, const Raw8<float>& b) {
+__device__ __forceinline__ void mma(f32x4& acc, const Floats& a, const Floats& b) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
 }
@@ -300,21 +319,21 @@ struct Stage {
     Raw4<S> turn[TR ? 8 : 1];
   };
   Unit r[kEach];
+  int inner;
 
-  // Inner values from ninner on are zero; rows from nrows on repeat a valid one
-  // (their products are never stored).  Whole pieces take loads without a branch,
-  // all of them in flight at once: a guarded load waits for the one before it.
+  // Rows from nrows on repeat a valid one (their products are never stored), inner
+  // values from ninner on too, and put makes those zero.  Whole pieces take loads
+  // without a branch or a use, all of them in flight at once: a guarded load waits
+  // for the one before it.
   __device__ __forceinline__ void fetch(const S* src, int64_t ld, int nrows, int ninner) {
+    inner = ninner;
     if constexpr (TR) {
       if (nrows >= ROWS || (nrows >= 4 && nrows % 4 == 0)) {
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
           const int u = unit(q), row = min(u % (ROWS / 4) * 4, nrows - 4), k = u / (ROWS / 4) * 8;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            r[q].turn[e] = load_n<S, 4>(src + min(k + e, ninner - 1) * ld + row);
-            if (k + e >= ninner) r[q].turn[e] = Raw4<S>{};
-          }
+          for (int e = 0; e < 8; ++e) r[q].turn[e] = load_n<S, 4>(src + min(k + e, ninner - 1) * ld + row);
         }
       } else {
 #pragma unroll
@@ -331,7 +350,6 @@ struct Stage {
         for (int q = 0; q < kEach; ++q) {
           const int u = unit(q), k = u % PIECES * 8, row = min(u / PIECES, nrows - 1);
           r[q].line = load8(src + row * ld + min(k, ninner - 8));
-          if (k >= ninner) r[q].line = Raw8<S>{};
         }
       } else {
 #pragma unroll
@@ -359,11 +377,13 @@ struct Stage {
         for (int a = 0; a < 4; ++a) {
           F f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r[q].turn[e].v[a]);
+          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, c * 8 + e < inner ? r[q].turn[e].get(a) : static_cast<S>(0.f));
           put_frag(lds, kPlane, c * (ROWS + 1) + row + a, f);
         }
       } else {
-        put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, frag_of<T, S>(r[q].line));
+        F f = frag_of<T, S>(r[q].line);
+        if (u % PIECES * 8 >= inner) f = F{};
+        put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, f);
       }
     }
   }
@@ -502,19 +522,21 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int b = 0; b < RK; ++b) {
     const int t = tok + n, i = b * 32 + g * 8;
-    Raw8<float> h = {};
+    float h[8] = {};
     if (t < tl.n) {
       const int64_t at = static_cast<int64_t>(tl.t0 + t) * rank + i;
       for (int p = 0; p < parts; ++p) {
         const Raw8<float> q = load8(H + p * sg.tokens * rank + at, rank - i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h.v[e] += q.v[e];
+        for (int e = 0; e < 8; ++e) h[e] += q.get(e);
       }
-      if (Hsum != nullptr && block == 0 && (NT == 4 || wave == 0)) store_n(Hsum + at, h, rank - i);
+      if (Hsum != nullptr && block == 0 && (NT == 4 || wave == 0))
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < rank) Hsum[at + e] = h[e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h.v[e] *= scale;
-    fh[b] = frag_of<T, float>(h);
+    for (int e = 0; e < 8; ++e) put_elem<T, float>(fh[b], e, h[e] * scale);
   }
   for (int j0 = c0; j0 < c1; j0 += COLS) {
     const int row = (NT == 1 ? wave * 64 : 0) + n * PC, j = j0 + row;    // this lane's columns
@@ -546,7 +568,7 @@ __global__ void __launch_bounds__(kThreads)
       const int t = tok + g * 4 + q;
       if (t >= tl.n) continue;
 #pragma unroll
-      for (int a = 0; a < PC; ++a) r[q].v[a] = from_f32<T>(to_f32(r[q].v[a]) + acc[a][q]);
+      for (int a = 0; a < PC; ++a) r[q].set(a, from_f32<T>(to_f32(r[q].get(a)) + acc[a][q]));
       store_n(out + (tl.t0 + t) * ldo + j, r[q], j0 + COLS <= c1 ? PC : c1 - j);
     }
   }
@@ -595,19 +617,18 @@ __global__ void __launch_bounds__(kThreads)
         SH sh;
         sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left);
         RawN<T, PC> cur[8], nxt[8];
-        auto fetch = [&](RawN<T, PC>(&q)[8], int b) {         // tokens of other segments enter as zeros
+        auto fetch = [&](RawN<T, PC>(&q)[8], int b) {
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int k = b * 32 + g * 8 + e;
               q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j);
-              if (k >= left) q[e] = RawN<T, PC>{};
             }
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int k = b * 32 + g * 8 + e;
-              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j, k < left ? valid : 0);
+              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j, valid);
             }
           }
         };
@@ -617,11 +638,15 @@ __global__ void __launch_bounds__(kThreads)
         __syncthreads();
         for (int b = 0; b * 32 < left; ++b) {
           if (b * 32 + 32 < left) fetch(nxt, b + 1);
+          if (b * 32 + 32 > left)                              // no tokens of other segments
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (b * 32 + g * 8 + e >= left) cur[e] = RawN<T, PC>{};
           Frag<T, T> fx[PC];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, cur[e].v[a]);
+            for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, cur[e].get(a));
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
             const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);

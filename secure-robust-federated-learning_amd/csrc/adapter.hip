@@ -83,28 +83,43 @@ __device__ __forceinline__ RawN<S, N> load_n(const S* p) {
   return r;
 }
 
-// the first `valid` of them, the rest zero
+// Elements o .. o + N - 1 of n >= N that lie one behind the other, where those
+// that do not matter may be others: the last N of all where o + N is beyond the
+// end, to be moved into place by settle when they are used.  So every lane's load
+// is one without a branch, and many are in flight at once.
 template <typename S, int N>
-__device__ __forceinline__ RawN<S, N> load_n(const S* p, int valid) {
-  if (valid >= N) return load_n<S, N>(p);
-  RawN<S, N> r = {};
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (e < valid) r.set(e, p[e]);
-  return r;
+__device__ __forceinline__ RawN<S, N> load_at(const S* p, int64_t o, int64_t n) {
+  return load_n<S, N>(p + min(o, n - N));
 }
 
-template <typename S>
-__device__ __forceinline__ Raw8<S> load8(const S* p) {
-  return load_n<S, 8>(p);
-}
-template <typename S>
-__device__ __forceinline__ Raw8<S> load8(const S* p, int valid) {
-  return load_n<S, 8>(p, valid);
-}
-template <typename S>
-__device__ __forceinline__ Raw4<S> load4(const S* p, int valid) {
-  return load_n<S, 4>(p, valid);
+template <typename S, int N>
+__device__ __forceinline__ void settle(RawN<S, N>& r, int64_t o, int64_t n) {
+  const int64_t d = o - (n - N);
+  if (__ballot(d > 0 && d < N) == 0) return;
+  const int by = d > 0 ? static_cast<int>(d) : 0;
+  constexpr int kWords = RawN<S, N>::kWords, kPer = 4 / sizeof(S);
+  auto words_down = [&](auto step) {                     // by a constant: registers have no address
+    constexpr int kStep = decltype(step)::value;
+    if constexpr (kStep < kWords) {
+      const bool on = (by & (kStep * kPer)) != 0;
+#pragma unroll
+      for (int e = 0; e + kStep < kWords; ++e) {
+        const unsigned from = r.w[e + kStep], at = r.w[e];
+        r.w[e] = on ? from : at;
+      }
+    }
+  };
+  words_down(std::integral_constant<int, 4>{});
+  words_down(std::integral_constant<int, 2>{});
+  words_down(std::integral_constant<int, 1>{});
+  if constexpr (sizeof(S) == 2) {
+    const bool on = (by & 1) != 0;
+#pragma unroll
+    for (int e = 0; e < kWords; ++e) {
+      const unsigned next = e + 1 < kWords ? r.w[e + 1] : 0u, at = r.w[e];
+      r.w[e] = on ? at >> 16 | next << 16 : at;
+    }
+  }
 }
 
 template <typename S, int N>
@@ -319,44 +334,26 @@ struct Stage {
     Raw4<S> turn[TR ? 8 : 1];
   };
   Unit r[kEach];
-  int inner;
+  int64_t ld, total;
+  int rows, inner;
 
-  // Rows from nrows on repeat a valid one (their products are never stored), inner
-  // values from ninner on too, and put makes those zero.  Whole pieces take loads
-  // without a branch or a use, all of them in flight at once: a guarded load waits
-  // for the one before it.
-  __device__ __forceinline__ void fetch(const S* src, int64_t ld, int nrows, int ninner) {
+  // `total` elements from src on may be read.  Rows from nrows on hold anything
+  // (their products are never stored), inner values from ninner on are zero once
+  // they are put.
+  __device__ __forceinline__ void fetch(const S* src, int64_t ld_, int nrows, int ninner, int64_t total_) {
+    ld = ld_;
+    total = total_;
+    rows = nrows;
     inner = ninner;
-    if constexpr (TR) {
-      if (nrows >= ROWS || (nrows >= 4 && nrows % 4 == 0)) {
 #pragma unroll
-        for (int q = 0; q < kEach; ++q) {
-          const int u = unit(q), row = min(u % (ROWS / 4) * 4, nrows - 4), k = u / (ROWS / 4) * 8;
+    for (int q = 0; q < kEach; ++q) {
+      const int u = unit(q);
+      if constexpr (TR) {
+        const int row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 8;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) r[q].turn[e] = load_n<S, 4>(src + min(k + e, ninner - 1) * ld + row);
-        }
+        for (int e = 0; e < 8; ++e) r[q].turn[e] = load_at<S, 4>(src, turn_at(k + e, row), total);
       } else {
-#pragma unroll
-        for (int q = 0; q < kEach; ++q) {
-          const int u = unit(q), row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 8;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            r[q].turn[e] = load4(src + (k + e) * ld + row, k + e < ninner ? nrows - row : 0);
-        }
-      }
-    } else {
-      if (ninner >= 8 * PIECES || (ninner >= 8 && ninner % 8 == 0)) {
-#pragma unroll
-        for (int q = 0; q < kEach; ++q) {
-          const int u = unit(q), k = u % PIECES * 8, row = min(u / PIECES, nrows - 1);
-          r[q].line = load8(src + row * ld + min(k, ninner - 8));
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < kEach; ++q) {
-          const int u = unit(q), k = u % PIECES * 8, row = min(u / PIECES, nrows - 1);
-          r[q].line = load8(src + row * ld + k, ninner - k);
-        }
+        r[q].line = load_at<S, 8>(src, line_at(u), total);
       }
     }
   }
@@ -366,24 +363,41 @@ struct Stage {
     return min(q * kThreads + static_cast<int>(threadIdx.x), kUnits - 1);
   }
 
-  __device__ __forceinline__ void put(u32x4* lds) const {
+  __device__ __forceinline__ int64_t turn_at(int k, int row) const { return min(k, inner - 1) * ld + row; }
+  __device__ __forceinline__ int64_t line_at(int u) const { return min(u / PIECES, rows - 1) * ld + u % PIECES * 8; }
+
+  __device__ __forceinline__ void put(u32x4* lds) {
+    // whether any load of this stage ended before its place
+    const bool near = TR ? turn_at(8 * PIECES, ROWS) > total : (rows - 1) * ld + 8 * PIECES > total;
 #pragma unroll
     for (int q = 0; q < kEach; ++q) {
-      const int u = q * kThreads + static_cast<int>(threadIdx.x);
-      if (kUnits % kThreads != 0 && u >= kUnits) continue;
+      const bool in = kUnits % kThreads == 0 || q * kThreads + static_cast<int>(threadIdx.x) < kUnits;
+      const int u = unit(q);
       if constexpr (TR) {
         const int row = u % (ROWS / 4) * 4, c = u / (ROWS / 4);
+        if (near)
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          F f;
+          for (int e = 0; e < 8; ++e) settle(r[q].turn[e], turn_at(c * 8 + e, row), total);
+        if (in)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, c * 8 + e < inner ? r[q].turn[e].get(a) : static_cast<S>(0.f));
-          put_frag(lds, kPlane, c * (ROWS + 1) + row + a, f);
-        }
+          for (int a = 0; a < 4; ++a) {
+            F f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              put_elem<T, S>(f, e, c * 8 + e < inner ? r[q].turn[e].get(a) : static_cast<S>(0.f));
+            put_frag(lds, kPlane, c * (ROWS + 1) + row + a, f);
+          }
       } else {
-        F f = frag_of<T, S>(r[q].line);
-        if (u % PIECES * 8 >= inner) f = F{};
-        put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, f);
+        const int k = u % PIECES * 8;
+        F f;
+        if (inner >= 8 * PIECES) {
+          f = frag_of<T, S>(r[q].line);
+        } else {
+          if (near) settle(r[q].line, line_at(u), total);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, k + e < inner ? r[q].line.get(e) : static_cast<S>(0.f));
+        }
+        if (in) put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, f);
       }
     }
   }
@@ -431,19 +445,19 @@ __global__ void __launch_bounds__(kThreads)
   f32x4 acc[RT] = {};
   SX sx;
   SW sw;
-  if (j0 < j1) {
-    sx.fetch(xs + j0, ldx, tl.n, j1 - j0);
-    sw.fetch(ws + (AT ? static_cast<int64_t>(j0) * rank : j0), wld, rank, j1 - j0);
-  }
+  const int64_t xall = (sg.tokens - 1 - tl.t0) * ldx + width, wall = static_cast<int64_t>(rank) * width;
+  auto fetch = [&](int j) {
+    const int64_t at = AT ? static_cast<int64_t>(j) * rank : j;
+    sx.fetch(xs + j, ldx, tl.n, j1 - j, xall - j);
+    sw.fetch(ws + at, wld, rank, j1 - j, wall - at);
+  };
+  if (j0 < j1) fetch(j0);
   for (int j = j0; j < j1; j += KB) {
     __syncthreads();
     sx.put(lds);
     sw.put(ldw_);
     __syncthreads();
-    if (j + KB < j1) {
-      sx.fetch(xs + j + KB, ldx, tl.n, j1 - j - KB);
-      sw.fetch(ws + (AT ? static_cast<int64_t>(j + KB) * rank : j + KB), wld, rank, j1 - j - KB);
-    }
+    if (j + KB < j1) fetch(j + KB);
 #pragma unroll
     for (int b = NT == 1 ? wave : 0; b < KB / 32; b += NT == 1 ? 4 : 1) {
       const auto fx = SX::get(lds, (NT == 1 ? 0 : wave * 16) + n, b * 4 + g);
@@ -500,6 +514,7 @@ __global__ void __launch_bounds__(kThreads)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   const int c0 = block * span, c1 = min(width, c0 + span);
+  const int64_t ball = (sg.tokens - 1) * ldb + width;    // elements of base
   if (tl.slot < 0) {
     if (Hsum != nullptr && block == 0)
       for (int i = threadIdx.x; i < tl.n * rank; i += kThreads) Hsum[static_cast<int64_t>(tl.t0) * rank + i] = 0.f;
@@ -508,15 +523,24 @@ __global__ void __launch_bounds__(kThreads)
       for (int j = c0 + lane * 8; j < c1; j += 512) {
         const int valid = min(8, c1 - j);
         Raw8<T> r = {};
-        if (base != nullptr) r = load8(base + (tl.t0 + t) * ldb + j, valid);
+        if (base != nullptr) {
+          const int64_t at = (tl.t0 + t) * ldb + j;
+          r = load_at<T, 8>(base, at, ball);
+          settle(r, at, ball);
+        }
         store_n(out + (tl.t0 + t) * ldo + j, r, valid);
       }
     return;
   }
   const W* ws = w + tl.slot * ldw;
   const int64_t wld = AT ? rank : width;
+  const int64_t wall = static_cast<int64_t>(rank) * width;
   SW sw;
-  sw.fetch(ws + (AT ? static_cast<int64_t>(c0) * rank : c0), wld, width - c0, rank);
+  auto fetch = [&](int j) {
+    const int64_t at = AT ? static_cast<int64_t>(j) * rank : j;
+    sw.fetch(ws + at, wld, width - j, rank, wall - at);
+  };
+  fetch(c0);
   const int tok = NT == 1 ? 0 : wave * 16;               // the wave's first token
   Frag<T, float> fh[RK];
 #pragma unroll
@@ -524,16 +548,17 @@ __global__ void __launch_bounds__(kThreads)
     const int t = tok + n, i = b * 32 + g * 8;
     float h[8] = {};
     if (t < tl.n) {
-      const int64_t at = static_cast<int64_t>(tl.t0 + t) * rank + i;
+      const int64_t at = static_cast<int64_t>(tl.t0 + t) * rank;
       for (int p = 0; p < parts; ++p) {
-        const Raw8<float> q = load8(H + p * sg.tokens * rank + at, rank - i);
+        // a load may take up to 7 floats behind the last part, which the workspace has
+        const Raw8<float> q = load_n<float, 8>(H + p * sg.tokens * rank + at + min(i, rank - 1));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] += q.get(e);
+        for (int e = 0; e < 8; ++e) h[e] += i + e < rank ? q.get(e) : 0.f;
       }
       if (Hsum != nullptr && block == 0 && (NT == 4 || wave == 0))
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (i + e < rank) Hsum[at + e] = h[e];
+          if (i + e < rank) Hsum[at + i + e] = h[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) put_elem<T, float>(fh[b], e, h[e] * scale);
@@ -541,23 +566,14 @@ __global__ void __launch_bounds__(kThreads)
   for (int j0 = c0; j0 < c1; j0 += COLS) {
     const int row = (NT == 1 ? wave * 64 : 0) + n * PC, j = j0 + row;    // this lane's columns
     RawN<T, PC> r[4] = {};
-    if (base != nullptr) {
-      const T* bp[4];
+    if (base != nullptr)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) bp[q] = base + (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j;
-      if (j0 + COLS <= c1) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] = load_n<T, PC>(bp[q]);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] = load_n<T, PC>(bp[q], c1 - j);
-      }
-    }
+      for (int q = 0; q < 4; ++q)
+        r[q] = load_at<T, PC>(base, (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j, ball);
     __syncthreads();
     sw.put(lds);
     __syncthreads();
-    if (j0 + COLS < c1)
-      sw.fetch(ws + (AT ? static_cast<int64_t>(j0 + COLS) * rank : j0 + COLS), wld, width - j0 - COLS, rank);
+    if (j0 + COLS < c1) fetch(j0 + COLS);
     f32x4 acc[PC] = {};
 #pragma unroll
     for (int b = 0; b < RK; ++b)
@@ -566,6 +582,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int t = tok + g * 4 + q;
+      if (base != nullptr && j0 + COLS > c1) settle(r[q], (tl.t0 + min(t, tl.n - 1)) * ldb + j, ball);
       if (t >= tl.n) continue;
 #pragma unroll
       for (int a = 0; a < PC; ++a) r[q].set(a, from_f32<T>(to_f32(r[q].get(a)) + acc[a][q]));
@@ -596,6 +613,7 @@ __global__ void __launch_bounds__(kThreads)
   const int c = blockIdx.y, j = ((static_cast<int>(blockIdx.x) * 4 + wave) * 16 + n) * PC;
   const int valid = max(0, min(PC, width - j));
   const bool whole = (static_cast<int>(blockIdx.x) + 1) * 64 * PC <= width;
+  const int64_t xall = (sg.tokens - 1) * ldx + width;      // elements of x
   const int turns = static_cast<int>(gridDim.z);
   f32x4 acc[RT][PC] = {};
   int turn = static_cast<int>(blockIdx.z);                 // stages until this part's next
@@ -615,22 +633,14 @@ __global__ void __launch_bounds__(kThreads)
         turn = turns - 1;
         const int left = min(kOuterTokens, t1 - t);
         SH sh;
-        sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left);
+        sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left, (sg.tokens - t) * rank);
         RawN<T, PC> cur[8], nxt[8];
+        auto x_at = [&](int b, int e) {
+          return static_cast<int64_t>(t + min(b * 32 + g * 8 + e, left - 1)) * ldx + j;
+        };
         auto fetch = [&](RawN<T, PC>(&q)[8], int b) {
-          if (whole) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int k = b * 32 + g * 8 + e;
-              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int k = b * 32 + g * 8 + e;
-              q[e] = load_n<T, PC>(x + static_cast<int64_t>(t + min(k, left - 1)) * ldx + j, valid);
-            }
-          }
+          for (int e = 0; e < 8; ++e) q[e] = load_at<T, PC>(x, x_at(b, e), xall);
         };
         fetch(cur, 0);
         __syncthreads();
@@ -638,6 +648,9 @@ __global__ void __launch_bounds__(kThreads)
         __syncthreads();
         for (int b = 0; b * 32 < left; ++b) {
           if (b * 32 + 32 < left) fetch(nxt, b + 1);
+          if (!whole)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) settle(cur[e], x_at(b, e), xall);
           if (b * 32 + 32 > left)                              // no tokens of other segments
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -702,6 +715,73 @@ __global__ void __launch_bounds__(256)
   *o = accumulate ? *o + scale * a : scale * a;
 }
 
+// ---------------------------------------------------------------------------
+// The same three products element by element, for rows of fewer than 8 values
+// (and outer for fewer than 8 hidden values), which the 16-byte loads above would
+// read beyond.
+// ---------------------------------------------------------------------------
+template <typename T, typename W>
+__global__ void __launch_bounds__(256)
+    tiny_shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, int64_t si,
+                       int64_t sj, Segs sg, int width, int rank, float* __restrict__ H) {
+  const int64_t t = blockIdx.x;
+  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i = wave; i < rank; i += 4) {
+    float a = 0.f;
+    if (c >= 0) {
+      for (int j = lane; j < width; j += 64) a += to_f32(w[c * ldw + i * si + j * sj]) * to_f32(x[t * ldx + j]);
+      for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
+    }
+    if (lane == 0) H[t * rank + i] = a;
+  }
+}
+
+template <typename T, typename W>
+__global__ void __launch_bounds__(256)
+    tiny_expand_kernel(const T* base, int64_t ldb, const float* __restrict__ H, const W* __restrict__ w, int64_t ldw,
+                       int64_t si, int64_t sj, Segs sg, int width, int rank, float scale, T* out, int64_t ldo) {
+  const int64_t t = blockIdx.x;
+  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t);
+  for (int j = threadIdx.x; j < width; j += 256) {
+    const float b = base != nullptr ? to_f32(base[t * ldb + j]) : 0.f;
+    float a = 0.f;
+    if (c >= 0)
+      for (int i = 0; i < rank; ++i) a += to_f32(w[c * ldw + i * si + j * sj]) * H[t * rank + i];
+    out[t * ldo + j] = from_f32<T>(c >= 0 ? b + scale * a : b);
+  }
+}
+
+__global__ void __launch_bounds__(256)
+    tiny_sum_kernel(const float* H, int parts, int64_t all, float* sum) {
+  const int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (q >= all) return;
+  float a = H[q];
+  for (int p = 1; p < parts; ++p) a += H[p * all + q];
+  sum[q] = a;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    tiny_outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
+                      float scale, float* __restrict__ G, int64_t ldg, int64_t si, int64_t sj, int accumulate) {
+  const int c = blockIdx.y;
+  const int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int j = static_cast<int>(q % width), i = static_cast<int>(q / width);
+  if (i >= rank) return;
+  float a = 0.f;
+  bool any = false;
+  for (int s = 0; s < sg.nseg; ++s) {
+    if (sg.slots[s] != c) continue;
+    const int t0 = seg_start(sg, s + 1), t1 = seg_start(sg, s + 2);
+    for (int t = t0; t < t1; ++t) a += H[static_cast<int64_t>(t) * rank + i] * to_f32(x[t * ldx + j]);
+    any |= t1 > t0;
+  }
+  float* g = G + c * ldg + i * si + j * sj;
+  if (!accumulate) *g = scale * a;
+  else if (any) *g += scale * a;
+}
+
 struct Shape {
   int64_t k, m;
   int rank;
@@ -747,10 +827,16 @@ static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
   return p;
 }
 
+// Columns a lane of outer takes: 8, or 4 where 8 leave fewer than two workgroups
+// a compute unit or (rank above 32) too few registers.
+static int outer_cols(int64_t width, int nslots, int rank) {
+  return rank <= 32 && cdiv(width, 64 * 8) * nslots >= 512 ? 8 : 4;
+}
+
 // Parts of a client's tokens that outer sums apart: two workgroups a compute
 // unit, each with at least 2 stages of tokens.
 static int outer_parts(int64_t tokens, int nslots, int64_t width, int rank) {
-  const int64_t blocks = cdiv(width, rank <= 32 ? 512 : 256) * nslots;
+  const int64_t blocks = cdiv(width, 64 * outer_cols(width, nslots, rank)) * nslots;
   const int64_t stages = cdiv(tokens, kOuterTokens * static_cast<int64_t>(nslots));
   int p = 1;
   while (p < kMaxParts && blocks * p < 512 && stages >= 4 * p) p *= 2;
@@ -766,8 +852,9 @@ static Workspace plan(int64_t tokens, int nseg, int nslots, int64_t k, int64_t m
   const int pa = outer_parts(tokens, nslots, k, rank), pb = outer_parts(tokens, nslots, m, rank);
   Workspace w{};
   w.h = 0;
-  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, nseg, k);
-  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, nseg, m) + 1);
+  // expand may load up to 7 floats behind the parts of h or z
+  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, nseg, k) + 32;
+  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, nseg, m) + 1) + 32;
   w.gb = w.ga + (pa > 1 ? static_cast<size_t>(pa) * nslots * k * row : 0);
   w.bytes = w.gb + (pb > 1 ? static_cast<size_t>(pb) * nslots * m * row : 0) + 16;
   return w;
@@ -788,6 +875,12 @@ static int with_tile(const Segs& sg, int rank, F&& f) {
 template <typename T, typename W, bool AT>
 static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw, const Segs& sg, int64_t width,
                          int parts, int rank, float* H, hipStream_t st) {
+  if (width < 8) {
+    hipLaunchKernelGGL((tiny_shrink_kernel<T, W>), dim3(static_cast<unsigned>(sg.tokens)), dim3(256), 0, st,
+                       static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, AT ? 1 : width,
+                       AT ? static_cast<int64_t>(rank) : 1, sg, static_cast<int>(width), rank, H);
+    return launch_status("tiny_shrink_kernel");
+  }
   return with_tile(sg, rank, [&](auto nt, auto rt) {
     constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, KB = kShrinkCols<T, RT, NT>;
     const int part = static_cast<int>(cdiv(cdiv(width, parts), KB) * KB);
@@ -802,6 +895,21 @@ template <typename T, typename W, bool AT>
 static int launch_expand(const void* base, int64_t ldb, const float* H, int parts, const void* w, int64_t ldw,
                          const Segs& sg, int64_t width, int rank, float scale, void* out, int64_t ldo, float* Hsum,
                          hipStream_t st) {
+  if (width < 8) {
+    if (parts > 1 || Hsum != nullptr) {
+      float* sum = Hsum != nullptr ? Hsum : const_cast<float*>(H);
+      const int64_t all = sg.tokens * rank;
+      hipLaunchKernelGGL(tiny_sum_kernel, dim3(static_cast<unsigned>(cdiv(all, 256))), dim3(256), 0, st, H, parts, all,
+                         sum);
+      if (int rc = launch_status("tiny_sum_kernel")) return rc;
+      H = sum;
+    }
+    hipLaunchKernelGGL((tiny_expand_kernel<T, W>), dim3(static_cast<unsigned>(sg.tokens)), dim3(256), 0, st,
+                       static_cast<const T*>(base), ldb, H, static_cast<const W*>(w), ldw, AT ? 1 : width,
+                       AT ? static_cast<int64_t>(rank) : 1, sg, static_cast<int>(width), rank, scale,
+                       static_cast<T*>(out), ldo);
+    return launch_status("tiny_expand_kernel");
+  }
   return with_tile(sg, rank, [&](auto nt, auto rt) {
     constexpr int NT = decltype(nt)::value, RK = decltype(rt)::value == 4 ? 2 : 1, COLS = kExpandCols<NT>;
     const int tiles = tile_count<16 * NT>(sg);
@@ -819,16 +927,30 @@ static int launch_expand(const void* base, int64_t ldb, const float* H, int part
 template <typename T, bool AT>
 static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& sg, int64_t width, int rank,
                         float scale, float* G, int64_t ldg, int accumulate, float* parts_ws, hipStream_t st) {
+  if (width < 8 || sg.tokens * rank < 8) {
+    const dim3 tg(static_cast<unsigned>(cdiv(rank * width, 256)), static_cast<unsigned>(sg.nslots));
+    hipLaunchKernelGGL((tiny_outer_kernel<T>), tg, dim3(256), 0, st, static_cast<const T*>(x), ldx, H, sg,
+                       static_cast<int>(width), rank, scale, G, ldg, AT ? 1 : width,
+                       AT ? static_cast<int64_t>(rank) : 1, accumulate);
+    return launch_status("tiny_outer_kernel");
+  }
   const int parts = outer_parts(sg.tokens, sg.nslots, width, rank);
   const int64_t per = rank * width, stride = per * sg.nslots;
-  const int rc = with_tile(sg, rank, [&](auto, auto rt) {
-    constexpr int RT = decltype(rt)::value, PC = RT == 4 ? 4 : 8;
+  auto go = [&](auto rt, auto pc) {
+    constexpr int RT = decltype(rt)::value, PC = decltype(pc)::value;
     const dim3 grid(static_cast<unsigned>(cdiv(width, 64 * PC)), static_cast<unsigned>(sg.nslots), parts);
     hipLaunchKernelGGL((outer_kernel<T, RT, PC, AT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx, H,
                        sg, static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg,
                        stride, accumulate);
     return launch_status("outer_kernel");
-  });
+  };
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, 2> two;
+  const std::integral_constant<int, 4> four;
+  const std::integral_constant<int, 8> eight;
+  const bool wide = outer_cols(width, sg.nslots, rank) == 8;
+  const int rc = rank > 32 ? go(four, four)
+                 : rank > 16 ? (wide ? go(two, eight) : go(two, four)) : (wide ? go(one, eight) : go(one, four));
   if (rc || parts == 1) return rc;
   const dim3 jg(static_cast<unsigned>(cdiv(per, 256)), static_cast<unsigned>(sg.nslots));
   hipLaunchKernelGGL((join_parts_kernel<AT>), jg, dim3(256), 0, st, parts_ws, parts, stride, sg,
@@ -847,10 +969,10 @@ template <typename T, typename W>
 static int run_apply(const void* base, int64_t ldbase, const void* x, int64_t ldx, const Weights& w, const Segs& sg,
                      const Shape& sh, void* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
   const int parts = shrink_parts(sg.tokens, sg.nseg, sh.k);
-  float* H = parts == 1 && hidden != nullptr ? hidden : reinterpret_cast<float*>(ws);
+  float* H = reinterpret_cast<float*>(ws);
   if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, parts, sh.rank, H, st)) return rc;
   return launch_expand<T, W, true>(base, ldbase, H, parts, w.B, w.ldb, sg, sh.m, sh.rank, sh.scale, out, ldo,
-                                   parts > 1 ? hidden : nullptr, st);
+                                   hidden, st);
 }
 
 struct GradOut {

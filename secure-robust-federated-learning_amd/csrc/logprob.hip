@@ -8,6 +8,8 @@
 //   s f + ...,  (u + s d) f + ...
 // so that  lse = m + log s,  logp = x_target - lse,  entropy = log s - u / s
 // without a difference of large numbers.
+#include <type_traits>
+
 #include "lm_common.hpp"
 
 namespace sra {
@@ -54,13 +56,30 @@ __device__ __forceinline__ void add_values(Stats& a, const float (&x)[N], float 
   }
 }
 
+// One wave-wide reduction by lane moves inside rows of 16 and between them; the
+// result is in lane 63 and returned to all.  `id` stands in for absent lanes.
+template <typename T, typename Op>
+__device__ __forceinline__ T wave_reduce(T v, T id, Op op) {
+  auto move = [&](auto ctrl, auto rows) {
+    const int m = __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, id), __builtin_bit_cast(int, v),
+                                              decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v = op(v, __builtin_bit_cast(T, m));
+  };
+  using I = std::integral_constant<int, 0xf>;
+  move(std::integral_constant<int, 0x111>{}, I{});       // from 1, 2, 4, 8 lanes below in the row
+  move(std::integral_constant<int, 0x112>{}, I{});
+  move(std::integral_constant<int, 0x114>{}, I{});
+  move(std::integral_constant<int, 0x118>{}, I{});
+  move(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});   // row ends to the next row
+  move(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});   // lane 31 to the upper half
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 __device__ __forceinline__ Stats wave_join(Stats a) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const Stats b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)};
-    join(a, b);
-  }
-  return a;
+  const float M = wave_reduce(a.m, kLowest, [](float p, float q) { return __builtin_elementwise_maximum(p, q); });
+  rescale(a, M);
+  auto add = [](float p, float q) { return p + q; };
+  return {M, wave_reduce(a.s, 0.f, add), wave_reduce(a.u, 0.f, add)};
 }
 
 // ---------------------------------------------------------------------------
@@ -125,47 +144,48 @@ __device__ __forceinline__ void top_offer(Top& t, int k, const unsigned (&key)[N
         be = e;
       }
     const int own = bi;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned ok = __shfl_xor(bk, o);
-      const int oi = __shfl_xor(bi, o);
-      if (before(ok, oi, bk, bi)) {
-        bk = ok;
-        bi = oi;
-      }
-    }
+    const unsigned mine = bk;
+    auto larger = [](unsigned p, unsigned q) { return max(p, q); };
+    bk = wave_reduce(mine, 0u, larger);
+    bi = static_cast<int>(~wave_reduce(mine == bk ? ~static_cast<unsigned>(own) : 0u, 0u, larger));
     if (bk == 0 || !before(bk, bi, t.kth, t.kth_idx)) return;
     top_insert(t, k, bk, bi);
-    if (be >= 0 && own == bi) live &= ~(1u << be);
+    if (be >= 0 && mine == bk && own == bi) live &= ~(1u << be);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Walk a row in index order: f(x[8], first index, valid) per lane, wave w of
-// nw taking every nw-th stretch of 512 from `from` to `to`.  16-byte loads from
-// the first aligned element on; the few elements before it and after the last
-// whole stretch go one by one through the same call.
+// Walk a row in index order: f(x[8], first index, valid) per lane, wave w of nw
+// taking every nw-th stretch of 512.  16-byte loads from the first aligned
+// element on; the few elements before it and after the last whole stretch go one
+// by one through the same call.
 // ---------------------------------------------------------------------------
 constexpr int kPer = 8;
 constexpr int kStretch = 64 * kPer;
 
+// 8 logits as they came, untouched until values takes them out
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[kPer]) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+struct Raw {
+  u32x4 v[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p) {
+  Raw<T> r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = a[e];
-      x[4 + e] = b[e];
-    }
-  } else {
-    union {
-      u32x4 v;
-      T t[kPer];
-    } q;
-    q.v = *reinterpret_cast<const u32x4*>(p);
+  for (int b = 0; b < static_cast<int>(sizeof(T) / 2); ++b) r.v[b] = reinterpret_cast<const u32x4*>(p)[b];
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void values(const Raw<T>& r, float (&x)[kPer]) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = to_f32(q.t[e]);
+  for (int e = 0; e < kPer; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      const unsigned word = r.v[e / 4][e % 4];       // a bit cast of the element itself takes the vector's first
+      x[e] = __builtin_bit_cast(float, word);
+    } else
+      x[e] = to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(r.v[0][e / 2] >> (e % 2 * 16))));
   }
 }
 
@@ -198,32 +218,59 @@ __device__ __forceinline__ int head_of(const T* row, int64_t n) {
   return static_cast<int>(min(static_cast<int64_t>(h), n));
 }
 
+// Stretches of 512 of a row, after the few elements before its first aligned one
+struct Span {
+  int head, body;          // first aligned index, whole stretches
+};
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const T* row, int n) {
+  const int h = head_of(row, n);
+  return {h, (n - h) / kStretch};
+}
+
+// the elements before the first and behind the last whole stretch
 template <typename T, typename F>
-__device__ __forceinline__ void walk(const T* row, int from, int to, int w, int nw, F&& f) {
+__device__ __forceinline__ void walk_head(const T* row, const Span& sp, int w, F&& f) {
+  if (w != 0 || sp.head == 0) return;            // at most 7, one a lane
   const int lane = threadIdx.x & 63;
-  const int h = from + head_of(row + from, to - from);
+  const bool in = lane < sp.head;
   float x[kPer];
-  if (w == 0 && h > from) {                      // at most 7 elements, one a lane
-    const bool in = from + lane < h;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = -__builtin_inff();
-    if (in) x[0] = to_f32(row[from + lane]);
-    f(x, from + lane, in ? 1 : 0);
-  }
-  const int body = (to - h) / kStretch;
-  for (int b = w; b < body; b += nw) {
-    const int i = h + b * kStretch + lane * kPer;
-    load8(row + i, x);
+  for (int e = 0; e < kPer; ++e) x[e] = -__builtin_inff();
+  if (in) x[0] = to_f32(row[lane]);
+  f(x, lane, in ? 1 : 0);
+}
+
+template <typename T, typename F>
+__device__ __forceinline__ void walk_tail(const T* row, int n, const Span& sp, int w, int nw, F&& f) {
+  const int t0 = sp.head + sp.body * kStretch;
+  if (t0 >= n || sp.body % nw != w) return;
+  const int i = t0 + (threadIdx.x & 63) * kPer;
+  const int valid = max(0, min(kPer, n - i));
+  float x[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) x[e] = e < valid ? to_f32(row[i + e]) : -__builtin_inff();
+  f(x, i, valid);
+}
+
+// the whole row, the next stretch's load in flight behind this one's work
+template <typename T, typename F>
+__device__ __forceinline__ void walk(const T* row, int n, int w, int nw, F&& f) {
+  const int lane = threadIdx.x & 63;
+  const Span sp = span_of(row, n);
+  walk_head(row, sp, w, f);
+  Raw<T> cur, nxt;
+  if (w < sp.body) cur = load8(row + sp.head + w * kStretch + lane * kPer);
+  for (int b = w; b < sp.body; b += nw) {
+    const int i = sp.head + b * kStretch + lane * kPer;
+    if (b + nw < sp.body) nxt = load8(row + i + nw * kStretch);
+    float x[kPer];
+    values(cur, x);
     f(x, i, kPer);
+    cur = nxt;
   }
-  const int t0 = h + body * kStretch;
-  if (t0 < to && body % nw == w) {               // the last, partial stretch
-    const int i = t0 + lane * kPer;
-    const int valid = max(0, min(kPer, to - i));
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = e < valid ? to_f32(row[i + e]) : -__builtin_inff();
-    f(x, i, valid);
-  }
+  walk_tail(row, n, sp, w, nw, f);
 }
 
 struct Args {
@@ -243,12 +290,15 @@ struct Args {
   int64_t ldg;
 };
 
-// the gradient of one row, given its lse and entropy
+// the gradient of 8 logits of a row, given its lse and entropy
 template <typename T>
-__device__ __forceinline__ void grad_row(const T* row, T* grow, int vocab, int64_t target, float lse, float ent,
-                                         float gl, float ge, int w, int nw) {
-  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
-  walk(row, 0, vocab, w, nw, [&](float (&x)[kPer], int i, int valid) {
+struct RowGrad {
+  T* grow;
+  int64_t target;
+  float lse, ent, gl, ge;
+  bool same;                // logits and gradient are aligned alike
+
+  __device__ __forceinline__ void operator()(float (&x)[kPer], int i, int valid) const {
     float g[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
@@ -266,11 +316,19 @@ __device__ __forceinline__ void grad_row(const T* row, T* grow, int vocab, int64
       for (int e = 0; e < kPer; ++e)
         if (e < valid) grow[i + e] = from_f32<T>(g[e]);
     }
-  });
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ RowGrad<T> row_grad(const T* row, T* grow, int64_t target, float lse, float ent, float gl,
+                                               float ge) {
+  return {grow, target, lse, ent, gl, ge,
+          ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0};
 }
 
-// WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.
-template <typename T, int WAVES, bool TOP, bool GRAD>
+// WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.  KEEP > 0: a wave
+// holds its up to KEEP stretches in registers from the one read to the gradient.
+template <typename T, int WAVES, bool TOP, bool GRAD, int KEEP>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
     logprob_kernel(const T* logits, Args a, T* grad) {
   static_assert(WAVES == 1 || WAVES >= 4, "a workgroup's waves share the barrier of one row");
@@ -278,7 +336,7 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
   __shared__ Stats sh_stats[kRows * WAVES];
   __shared__ unsigned sh_key[TOP ? kRows * WAVES * SRA_TOKEN_MAX_TOP : 1];
   __shared__ int sh_idx[TOP ? kRows * WAVES * SRA_TOKEN_MAX_TOP : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int local = wave / WAVES, w = wave % WAVES;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + local;
   const bool live = r < a.rows;
@@ -287,21 +345,39 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
   Top t;
   top_clear(t);
   const T* row = logits + (live ? r : 0) * a.ldl;
-  if (live) {
-    walk(row, 0, a.vocab, w, WAVES, [&](float (&x)[kPer], int i, int valid) {
-      float mx = x[0];
+  auto take = [&](float (&x)[kPer], int i, int valid) {
+    float mx = x[0];
 #pragma unroll
-      for (int e = 1; e < kPer; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
-      add_values(st, x, mx);
-      if constexpr (TOP) {
-        if (__ballot(t.kth == 0 || !(mx <= t.thr)) != 0) {
-          unsigned key[kPer];
+    for (int e = 1; e < kPer; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
+    add_values(st, x, mx);
+    if constexpr (TOP) {
+      if (__ballot(t.kth == 0 || !(mx <= t.thr)) != 0) {
+        unsigned key[kPer];
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) key[e] = key_of(x[e]);
-          top_offer(t, a.top, key, [&](int e) { return i + e; }, (1u << valid) - 1u);
-        }
+        for (int e = 0; e < kPer; ++e) key[e] = key_of(x[e]);
+        top_offer(t, a.top, key, [&](int e) { return i + e; }, (1u << valid) - 1u);
       }
-    });
+    }
+  };
+  Raw<T> kept[KEEP > 0 ? KEEP : 1];
+  const Span sp = span_of(row, a.vocab);
+  if (live) {
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q)
+        if (w + q * WAVES < sp.body) kept[q] = load8(row + sp.head + (w + q * WAVES) * kStretch + lane * kPer);
+      walk_head(row, sp, w, take);
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q)
+        if (w + q * WAVES < sp.body) {
+          float x[kPer];
+          values(kept[q], x);
+          take(x, sp.head + (w + q * WAVES) * kStretch + lane * kPer, kPer);
+        }
+      walk_tail(row, a.vocab, sp, w, WAVES, take);
+    } else {
+      walk(row, a.vocab, w, WAVES, take);
+    }
   }
   st = wave_join(st);
   if constexpr (WAVES > 1) {
@@ -314,15 +390,25 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
     }
     __syncthreads();
     // every wave joins them in the same order
-    st = sh_stats[local * WAVES];
-    for (int q = 1; q < WAVES; ++q) join(st, sh_stats[local * WAVES + q]);
+    st = sh_stats[0];
+#pragma unroll
+    for (int q = 1; q < WAVES; ++q) join(st, sh_stats[q]);
     if constexpr (TOP) {
-      if (w == 0)
-        for (int q = 1; q < WAVES; ++q) {
-          const unsigned key[1] = {lane < a.top ? sh_key[(wave + q) * SRA_TOKEN_MAX_TOP + lane] : 0u};
-          const int idx = lane < a.top ? sh_idx[(wave + q) * SRA_TOKEN_MAX_TOP + lane] : 0x7fffffff;
-          top_offer(t, a.top, key, [&](int) { return idx; }, 1u);
+      if (w == 0) {
+        // all lists at once: entry e of a lane is number e * 64 + lane
+        constexpr int kAll = WAVES * SRA_TOKEN_MAX_TOP / 64;
+        unsigned key[kAll];
+        int idx[kAll];
+#pragma unroll
+        for (int e = 0; e < kAll; ++e) {
+          const int q = e * 64 + lane, from = q / a.top * SRA_TOKEN_MAX_TOP + q % a.top;
+          const bool in = q < WAVES * a.top;
+          key[e] = in ? sh_key[from] : 0u;
+          idx[e] = in ? sh_idx[from] : 0x7fffffff;
         }
+        top_clear(t);
+        top_offer(t, a.top, key, [&](int e) { return idx[e]; }, (1u << kAll) - 1u);
+      }
     }
   }
   if (!live) return;
@@ -353,9 +439,22 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
   if constexpr (GRAD) {
     // the target is read before an in-place gradient replaces it
     if constexpr (WAVES > 1) __syncthreads(); else __threadfence_block();
-    const float gl = ignored || bad ? 0.f : a.grad_logp[r];
-    const float ge = a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f;
-    grad_row(row, grad + r * a.ldg, a.vocab, ignored || bad ? -1 : target, lse, ent, gl, ge, w, WAVES);
+    const bool none = ignored || bad;
+    const auto put = row_grad(row, grad + r * a.ldg, none ? -1 : target, lse, ent, none ? 0.f : a.grad_logp[r],
+                              a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f);
+    if constexpr (KEEP > 0) {
+      walk_head(row, sp, w, put);
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q)
+        if (w + q * WAVES < sp.body) {
+          float x[kPer];
+          values(kept[q], x);
+          put(x, sp.head + (w + q * WAVES) * kStretch + lane * kPer, kPer);
+        }
+      walk_tail(row, a.vocab, sp, w, WAVES, put);
+    } else {
+      walk(row, a.vocab, w, WAVES, put);
+    }
   }
 }
 
@@ -379,8 +478,9 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const T* logits, Args
   }
   const float ge = a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f;
   const float ent = a.grad_entropy != nullptr ? entropy[r] : 0.f;
-  grad_row(logits + r * a.ldl + from, grad + r * a.ldg + from, n, target - from, lse[r], ent, gl, ge,
-           threadIdx.x >> 6, 4);
+  const T* row = logits + r * a.ldl + from;
+  walk(row, n, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 4,
+       row_grad(row, grad + r * a.ldg + from, target - from, lse[r], ent, gl, ge));
 }
 
 static int check_logits(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
@@ -410,21 +510,38 @@ static int check_grad(const void* logits, int64_t ldl, const void* grad, int64_t
   return SRA_OK;
 }
 
-template <typename T, int WAVES>
+template <typename T, int WAVES, int KEEP>
 static int launch_rows(const void* logits, const Args& a, void* grad, hipStream_t st) {
   constexpr int kRows = WAVES < 4 ? 4 / WAVES : 1;
   const dim3 grid(static_cast<unsigned>(cdiv(a.rows, kRows))), block(WAVES < 4 ? 256 : WAVES * 64);
   const T* l = static_cast<const T*>(logits);
   T* g = static_cast<T*>(grad);
-  if (a.top > 0 && g != nullptr)
-    hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, true>), grid, block, 0, st, l, a, g);
-  else if (a.top > 0)
-    hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, false>), grid, block, 0, st, l, a, g);
-  else if (g != nullptr)
-    hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, true>), grid, block, 0, st, l, a, g);
-  else
-    hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, false>), grid, block, 0, st, l, a, g);
+  if (g != nullptr) {
+    if (a.top > 0)
+      hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, true, KEEP>), grid, block, 0, st, l, a, g);
+    else
+      hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, true, KEEP>), grid, block, 0, st, l, a, g);
+  } else if constexpr (KEEP == 0) {
+    if (a.top > 0)
+      hipLaunchKernelGGL((logprob_kernel<T, WAVES, true, false, 0>), grid, block, 0, st, l, a, g);
+    else
+      hipLaunchKernelGGL((logprob_kernel<T, WAVES, false, false, 0>), grid, block, 0, st, l, a, g);
+  }
   return launch_status("logprob_kernel");
+}
+
+// Waves a row: one for rows of up to 2048 logits; 4 where the rows fill the card,
+// 16 where they do not.  With the gradient, 8 waves keep a row of up to 65536
+// 16-bit (32768 float32) logits in registers; longer ones are read twice.
+template <typename T>
+static int launch(const void* logits, const Args& a, void* grad, hipStream_t st) {
+  constexpr int kMost = sizeof(T) == 4 ? 8 : 16;
+  if (a.vocab <= 2048) return launch_rows<T, 1, 0>(logits, a, grad, st);
+  if (grad != nullptr && a.vocab <= 8 * kMost * kStretch) {
+    if (a.vocab <= 8 * kMost / 4 * kStretch) return launch_rows<T, 8, kMost / 4>(logits, a, grad, st);
+    return launch_rows<T, 8, kMost>(logits, a, grad, st);
+  }
+  return a.rows < 1024 ? launch_rows<T, 16, 0>(logits, a, grad, st) : launch_rows<T, 4, 0>(logits, a, grad, st);
 }
 
 template <typename F>
@@ -467,7 +584,7 @@ extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype
   const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, top, logp, entropy, lse, top_logp, top_ids,
                grad_logp, grad_entropy, ldg};
   return with_type(dtype, [&](auto t) {
-    return launch_rows<decltype(t), 4>(logits, a, grad, static_cast<hipStream_t>(stream));
+    return launch<decltype(t)>(logits, a, grad, static_cast<hipStream_t>(stream));
   });
 }
 

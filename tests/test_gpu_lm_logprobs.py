@@ -50,8 +50,11 @@ def check(x, t, top, dtype, seed=0):
         wg, bound = ref.logits_grad(want, t, gl, gent, dtype)
         both, grad = lm.token_logprobs_and_grad(x, t, gl, gent, top=top, entropy=True)
         ref.within("grad", grad, wg, bound)
-        for a, b in zip(both, res):
-            assert torch.equal(a, b)
+        # another number of waves may sum the row in another order
+        ref.within("lse with grad", both.lse, want["lse"], want["e_lse"])
+        ref.within("logp with grad", both.logp, want["logp"], want["e_logp"])
+        ref.within("entropy with grad", both.entropy, want["ent"], want["e_ent"])
+        assert torch.equal(both.top_ids, res.top_ids)
         grad2 = lm.token_logprobs_grad(x, t, res.lse, gl, res.entropy, gent)
         ref.within("grad from lse", grad2, wg, bound)
     return res
@@ -60,7 +63,7 @@ def check(x, t, top, dtype, seed=0):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("R,V,top", [(1, 1, 1), (1, 2, 2), (3, 7, 5), (5, 64, 32), (4, 65, 0), (130, 10, 3),
                                      (3, 511, 1), (2, 512, 20), (2, 513, 20), (3, 2055, 7), (9, 5003, 4),
-                                     (1, 40001, 5), (2, 20000, 32)])
+                                     (1, 40001, 5), (2, 20000, 32), (2, 70001, 3), (1030, 2100, 2)])
 def test_rows(R, V, top, dtype):
     x, t = make(R, V, DT[dtype])
     check(x, t, min(top, V), DT[dtype])
@@ -157,17 +160,16 @@ def test_ignored_and_bad_targets():
     assert engine.row_fault_count(reset=True) == 2 and not g[[2, 3]].any()
 
 
-@pytest.mark.parametrize("V", [10, 777, 4100, 40001])
+@pytest.mark.parametrize("V", [10, 777, 4100, 40001, 66001])
 def test_gradient_in_place(V):
     x, t = make(7, V, torch.bfloat16)
     gl, ge = torch.full((7,), -0.25, device="cuda"), torch.full((7,), 0.5, device="cuda")
-    res, want = lm.token_logprobs_and_grad(x, t, gl, ge)
+    res, want = lm.token_logprobs_and_grad(x, t, gl, ge, entropy=True)
     y = x.clone()
     res2, got = lm.token_logprobs_and_grad(y, t, gl, ge, out=y)
     assert got.data_ptr() == y.data_ptr() and torch.equal(y, want) and torch.equal(res2.logp, res.logp)
     y = x.clone()
-    ent = lm.token_logprobs(x, t, entropy=True).entropy
-    lm.token_logprobs_grad(y, t, res.lse, gl, ent, ge, out=y)
+    lm.token_logprobs_grad(y, t, res.lse, gl, res.entropy, ge, out=y)
     # the same formula with the same lse and entropy
     assert torch.equal(y, want)
     wide = torch.full((7, V + 3), 7.0, dtype=torch.bfloat16, device="cuda")

@@ -412,9 +412,10 @@ struct Stage {
 // ---------------------------------------------------------------------------
 // shrink: H[t, i] = sum_j W[i, j] x[t, j].  A workgroup takes a tile of 16 NT
 // tokens and one of `parts` parts of the width, a stage of KB columns at a time.
-// NT 4: a wave a token group, all of them on the one staged weight.  NT 1 (short
-// segments, where the weight is the traffic): the waves share the stage's columns
-// and their sums meet in LDS in a fixed order.  W is [i][j] (AT false) or [j][i].
+// NT 4: a wave a token group and all ranks, or (ranks above 16) two token groups
+// and half of the ranks, which reads the least from LDS.  NT 1 (short segments,
+// where the weight is the traffic): the waves share the stage's columns and their
+// sums meet in LDS in a fixed order.  W is [i][j] (AT false) or [j][i].
 // ---------------------------------------------------------------------------
 template <typename T, int RT, int NT>
 constexpr int kShrinkCols = NT == 1 ? 512 / RT : (RT == 4 || kPlanes<Frag<T, T>> == 2) ? 128 : 256;
@@ -442,7 +443,9 @@ __global__ void __launch_bounds__(kThreads)
   const T* xs = x + static_cast<int64_t>(tl.t0) * ldx;
   const W* ws = w + tl.slot * ldw;
   const int64_t wld = AT ? rank : width;
-  f32x4 acc[RT] = {};
+  constexpr int RW = NT == 4 && RT >= 2 ? 2 : 1, UT = RW, UR = RT / RW;   // a wave's token groups and rank tiles
+  const int tok = NT == 1 ? 0 : wave / RW * UT * 16, rk = NT == 1 ? 0 : wave % RW * UR;
+  f32x4 acc[UT][UR] = {};
   SX sx;
   SW sw;
   const int64_t xall = (sg.tokens - 1 - tl.t0) * ldx + width, wall = static_cast<int64_t>(rank) * width;
@@ -460,30 +463,39 @@ __global__ void __launch_bounds__(kThreads)
     if (j + KB < j1) fetch(j + KB);
 #pragma unroll
     for (int b = NT == 1 ? wave : 0; b < KB / 32; b += NT == 1 ? 4 : 1) {
-      const auto fx = SX::get(lds, (NT == 1 ? 0 : wave * 16) + n, b * 4 + g);
+      Frag<T, T> fx[UT];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) mma(acc[r], SW::get(ldw_, r * 16 + n, b * 4 + g), fx);
+      for (int u = 0; u < UT; ++u) fx[u] = SX::get(lds, tok + u * 16 + n, b * 4 + g);
+#pragma unroll
+      for (int r = 0; r < UR; ++r) {
+        const auto fw = SW::get(ldw_, (rk + r) * 16 + n, b * 4 + g);
+#pragma unroll
+        for (int u = 0; u < UT; ++u) mma(acc[u][r], fw, fx[u]);
+      }
     }
   }
   if constexpr (NT == 1) {
     f32x4* sums = reinterpret_cast<f32x4*>(lds);
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RT; ++r) sums[(wave * RT + r) * 64 + lane] = acc[r];
+    for (int r = 0; r < RT; ++r) sums[(wave * RT + r) * 64 + lane] = acc[0][r];
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
     for (int r = 0; r < RT; ++r)
-      for (int q = 1; q < 4; ++q) acc[r] += sums[(q * RT + r) * 64 + lane];
+      for (int q = 1; q < 4; ++q) acc[0][r] += sums[(q * RT + r) * 64 + lane];
   }
-  const int t = (NT == 1 ? 0 : wave * 16) + n;
-  if (t >= tl.n) return;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int i = r * 16 + g * 4;
+  for (int u = 0; u < UT; ++u) {
+    const int t = tok + u * 16 + n;
+    if (t >= tl.n) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < rank) Hp[static_cast<int64_t>(t) * rank + i + e] = acc[r][e];
+    for (int r = 0; r < UR; ++r) {
+      const int i = (rk + r) * 16 + g * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < rank) Hp[static_cast<int64_t>(t) * rank + i + e] = acc[u][r][e];
+    }
   }
 }
 
@@ -500,13 +512,13 @@ __global__ void __launch_bounds__(kThreads)
 template <int NT>
 constexpr int kExpandCols = NT == 1 ? 256 : 128;
 
-template <typename T, typename W, int RK, int NT, bool AT>
+template <typename T, typename W, int RP, int NT, bool AT>
 __global__ void __launch_bounds__(kThreads)
     expand_kernel(const T* base, int64_t ldb, const float* __restrict__ H, int parts, const W* __restrict__ w,
                   int64_t ldw, Segs sg, int width, int blocks, int span, int rank, float scale, T* out, int64_t ldo,
                   float* __restrict__ Hsum) {
-  constexpr int COLS = kExpandCols<NT>, PC = NT == 1 ? 4 : 8;
-  using SW = Stage<T, W, COLS, RK * 4, !AT>;
+  constexpr int COLS = kExpandCols<NT>, PC = NT == 1 ? 4 : 8, RK = (RP + 3) / 4;
+  using SW = Stage<T, W, COLS, RP, !AT>;                 // RP pieces of 8 ranks
   __shared__ u32x4 lds[SW::kBytes / 16];
   const int tile = static_cast<int>(blockIdx.x) / blocks, block = static_cast<int>(blockIdx.x) % blocks;
   const Tile tl = find_tile<16 * NT>(sg, tile);
@@ -563,30 +575,44 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int e = 0; e < 8; ++e) put_elem<T, float>(fh[b], e, h[e] * scale);
   }
-  for (int j0 = c0; j0 < c1; j0 += COLS) {
-    const int row = (NT == 1 ? wave * 64 : 0) + n * PC, j = j0 + row;    // this lane's columns
-    RawN<T, PC> r[4] = {};
-    if (base != nullptr)
+  const int row = (NT == 1 ? wave * 64 : 0) + n * PC;    // this lane's columns of a stage
+  auto base_at = [&](int q, int j0) { return (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j0 + row; };
+  RawN<T, PC> r[4] = {}, nxt[4] = {};
+  if (base != nullptr)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        r[q] = load_at<T, PC>(base, (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j, ball);
+    for (int q = 0; q < 4; ++q) r[q] = load_at<T, PC>(base, base_at(q, c0), ball);
+  for (int j0 = c0; j0 < c1; j0 += COLS) {
+    const int j = j0 + row;
     __syncthreads();
     sw.put(lds);
     __syncthreads();
-    if (j0 + COLS < c1) fetch(j0 + COLS);
+    if (j0 + COLS < c1) {
+      fetch(j0 + COLS);
+      if (base != nullptr)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) nxt[q] = load_at<T, PC>(base, base_at(q, j0 + COLS), ball);
+    }
     f32x4 acc[PC] = {};
 #pragma unroll
     for (int b = 0; b < RK; ++b)
 #pragma unroll
-      for (int a = 0; a < PC; ++a) mma(acc[a], fh[b], SW::get(lds, row + a, b * 4 + g));
+      for (int a = 0; a < PC; ++a) {
+        // with fewer than 4 pieces the lanes of the others read the last one again: their h is 0,
+        // and so are their weights
+        Frag<T, W> fw = SW::get(lds, row + a, RP < 4 ? min(g, RP - 1) : b * 4 + g);
+        if (RP < 4 && g >= RP) fw = Frag<T, W>{};
+        mma(acc[a], fh[b], fw);
+      }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int t = tok + g * 4 + q;
-      if (base != nullptr && j0 + COLS > c1) settle(r[q], (tl.t0 + min(t, tl.n - 1)) * ldb + j, ball);
-      if (t >= tl.n) continue;
+      if (base != nullptr && j0 + COLS > c1) settle(r[q], base_at(q, j0), ball);
+      if (t < tl.n) {
 #pragma unroll
-      for (int a = 0; a < PC; ++a) r[q].set(a, from_f32<T>(to_f32(r[q].get(a)) + acc[a][q]));
-      store_n(out + (tl.t0 + t) * ldo + j, r[q], j0 + COLS <= c1 ? PC : c1 - j);
+        for (int a = 0; a < PC; ++a) r[q].set(a, from_f32<T>(to_f32(r[q].get(a)) + acc[a][q]));
+        store_n(out + (tl.t0 + t) * ldo + j, r[q], j0 + COLS <= c1 ? PC : c1 - j);
+      }
+      r[q] = nxt[q];
     }
   }
 }
@@ -601,12 +627,47 @@ __global__ void __launch_bounds__(kThreads)
 // rank * width) for join_parts.
 // ---------------------------------------------------------------------------
 constexpr int kOuterTokens = 128;
+constexpr int kOuterCols = 4;
 
-template <typename T, int RT, int PC, bool AT>
+// the stages of a slot's tokens, segment by segment; every `turns`-th is this part's
+struct SlotStages {
+  const Segs& sg;
+  int c, turn, turns;
+  int s0 = -64, t = 0, t1 = 0;
+  unsigned long long hits = 0;
+  bool any = false;
+
+  __device__ __forceinline__ bool next(int& at, int& left) {
+    while (true) {
+      for (; t < t1; t += kOuterTokens) {
+        if (turn-- != 0) continue;
+        turn = turns - 1;
+        at = t;
+        left = min(kOuterTokens, t1 - t);
+        t += kOuterTokens;
+        return true;
+      }
+      while (hits == 0) {
+        s0 += 64;
+        if (s0 >= sg.nseg) return false;
+        const int s = s0 + static_cast<int>(threadIdx.x & 63);
+        hits = __ballot(s < sg.nseg && sg.slots[min(s, sg.nseg - 1)] == c);
+      }
+      const int s = s0 + __ffsll(hits) - 1;
+      hits &= hits - 1;
+      t = seg_start(sg, s + 1);
+      t1 = seg_start(sg, s + 2);
+      any |= t1 > t;
+    }
+  }
+};
+
+template <typename T, int RT, bool AT>
 __global__ void __launch_bounds__(kThreads)
     outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
                  float scale, float* __restrict__ G, int64_t ldg, int64_t part_stride, int accumulate) {
   using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true>;
+  constexpr int PC = kOuterCols;
   __shared__ u32x4 lds[SH::kBytes / 16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
@@ -616,62 +677,59 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t xall = (sg.tokens - 1) * ldx + width;      // elements of x
   const int turns = static_cast<int>(gridDim.z);
   f32x4 acc[RT][PC] = {};
-  int turn = static_cast<int>(blockIdx.z);                 // stages until this part's next
-  bool any = false;
-  for (int s0 = 0; s0 < sg.nseg; s0 += 64) {
-    unsigned long long hits = __ballot(s0 + lane < sg.nseg && sg.slots[min(s0 + lane, sg.nseg - 1)] == c);
-    for (; hits != 0; hits &= hits - 1) {
-      const int s = s0 + __ffsll(hits) - 1;
-      const int t0 = seg_start(sg, s + 1), t1 = seg_start(sg, s + 2);
-      if (t1 <= t0) continue;
-      any = true;
-      for (int t = t0; t < t1; t += kOuterTokens) {
-        if (turn != 0) {
-          --turn;
-          continue;
-        }
-        turn = turns - 1;
-        const int left = min(kOuterTokens, t1 - t);
-        SH sh;
-        sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left, (sg.tokens - t) * rank);
-        RawN<T, PC> cur[8], nxt[8];
-        auto x_at = [&](int b, int e) {
-          return static_cast<int64_t>(t + min(b * 32 + g * 8 + e, left - 1)) * ldx + j;
-        };
-        auto fetch = [&](RawN<T, PC>(&q)[8], int b) {
+  SlotStages it{sg, c, static_cast<int>(blockIdx.z), turns};
+  SH sh;
+  RawN<T, PC> q[kOuterTokens / 32][8];
+  int t, left;
+  bool more = it.next(t, left);
+  auto x_at = [&](int b, int e) { return static_cast<int64_t>(t + min(b * 32 + g * 8 + e, left - 1)) * ldx + j; };
+  auto fetch = [&](int b) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q[e] = load_at<T, PC>(x, x_at(b, e), xall);
-        };
-        fetch(cur, 0);
-        __syncthreads();
-        sh.put(lds);
-        __syncthreads();
-        for (int b = 0; b * 32 < left; ++b) {
-          if (b * 32 + 32 < left) fetch(nxt, b + 1);
-          if (!whole)
+    for (int e = 0; e < 8; ++e) q[b][e] = load_at<T, PC>(x, x_at(b, e), xall);
+  };
+  auto fetch_h = [&] {
+    sh.fetch(H + static_cast<int64_t>(t) * rank, rank, rank, left, (sg.tokens - t) * rank);
+  };
+  if (more) {
+    fetch_h();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) settle(cur[e], x_at(b, e), xall);
-          if (b * 32 + 32 > left)                              // no tokens of other segments
+    for (int b = 0; b < kOuterTokens / 32; ++b)
+      if (b * 32 < left) fetch(b);
+  }
+  while (more) {
+    __syncthreads();
+    sh.put(lds);
+    __syncthreads();
+    const int t_now = t, left_now = left;
+    more = it.next(t, left);
+    if (more) fetch_h();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (b * 32 + g * 8 + e >= left) cur[e] = RawN<T, PC>{};
-          Frag<T, T> fx[PC];
+    for (int b = 0; b < kOuterTokens / 32; ++b) {
+      if (b * 32 < left_now) {
+        if (!whole)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
+            settle(q[b][e], static_cast<int64_t>(t_now + min(b * 32 + g * 8 + e, left_now - 1)) * ldx + j, xall);
+        if (b * 32 + 32 > left_now)                          // no tokens of other segments
 #pragma unroll
-            for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, cur[e].get(a));
+          for (int e = 0; e < 8; ++e)
+            if (b * 32 + g * 8 + e >= left_now) q[b][e] = RawN<T, PC>{};
+        Frag<T, T> fx[PC];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);
+        for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int a = 0; a < PC; ++a) mma(acc[r][a], fh, fx[a]);
-          }
+          for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, q[b][e].get(a));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) cur[e] = nxt[e];
+        for (int r = 0; r < RT; ++r) {
+          const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);
+#pragma unroll
+          for (int a = 0; a < PC; ++a) mma(acc[r][a], fh, fx[a]);
         }
       }
+      if (more && b * 32 < left) fetch(b);                   // the next stage's into the registers just read
     }
   }
+  const bool any = it.any;
   const bool last = gridDim.z == 1;
   if (last && accumulate && !any) return;
   const bool add = last && accumulate;
@@ -827,16 +885,10 @@ static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
   return p;
 }
 
-// Columns a lane of outer takes: 8, or 4 where 8 leave fewer than two workgroups
-// a compute unit or (rank above 32) too few registers.
-static int outer_cols(int64_t width, int nslots, int rank) {
-  return rank <= 32 && cdiv(width, 64 * 8) * nslots >= 512 ? 8 : 4;
-}
-
 // Parts of a client's tokens that outer sums apart: two workgroups a compute
 // unit, each with at least 2 stages of tokens.
-static int outer_parts(int64_t tokens, int nslots, int64_t width, int rank) {
-  const int64_t blocks = cdiv(width, 64 * outer_cols(width, nslots, rank)) * nslots;
+static int outer_parts(int64_t tokens, int nslots, int64_t width) {
+  const int64_t blocks = cdiv(width, 64 * kOuterCols) * nslots;
   const int64_t stages = cdiv(tokens, kOuterTokens * static_cast<int64_t>(nslots));
   int p = 1;
   while (p < kMaxParts && blocks * p < 512 && stages >= 4 * p) p *= 2;
@@ -849,7 +901,7 @@ struct Workspace {
 
 static Workspace plan(int64_t tokens, int nseg, int nslots, int64_t k, int64_t m, int rank) {
   const size_t row = static_cast<size_t>(rank) * 4;
-  const int pa = outer_parts(tokens, nslots, k, rank), pb = outer_parts(tokens, nslots, m, rank);
+  const int pa = outer_parts(tokens, nslots, k), pb = outer_parts(tokens, nslots, m);
   Workspace w{};
   w.h = 0;
   // expand may load up to 7 floats behind the parts of h or z
@@ -911,16 +963,21 @@ static int launch_expand(const void* base, int64_t ldb, const float* H, int part
     return launch_status("tiny_expand_kernel");
   }
   return with_tile(sg, rank, [&](auto nt, auto rt) {
-    constexpr int NT = decltype(nt)::value, RK = decltype(rt)::value == 4 ? 2 : 1, COLS = kExpandCols<NT>;
+    constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, COLS = kExpandCols<NT>;
     const int tiles = tile_count<16 * NT>(sg);
     // four workgroups a compute unit where the width allows it
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, tiles), cdiv(width, COLS)));
     const int span = static_cast<int>(cdiv(cdiv(width, want), COLS) * COLS);
     const int blocks = static_cast<int>(cdiv(width, span));
-    hipLaunchKernelGGL((expand_kernel<T, W, RK, NT, AT>), dim3(static_cast<unsigned>(tiles) * blocks), dim3(kThreads),
-                       0, st, static_cast<const T*>(base), ldb, H, parts, static_cast<const W*>(w), ldw, sg,
-                       static_cast<int>(width), blocks, span, rank, scale, static_cast<T*>(out), ldo, Hsum);
-    return launch_status("expand_kernel");
+    auto go = [&](auto rp) {
+      constexpr int RP = decltype(rp)::value;
+      hipLaunchKernelGGL((expand_kernel<T, W, RP, NT, AT>), dim3(static_cast<unsigned>(tiles) * blocks),
+                         dim3(kThreads), 0, st, static_cast<const T*>(base), ldb, H, parts, static_cast<const W*>(w),
+                         ldw, sg, static_cast<int>(width), blocks, span, rank, scale, static_cast<T*>(out), ldo, Hsum);
+      return launch_status("expand_kernel");
+    };
+    if constexpr (RT == 1) return rank <= 8 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
+    else return go(std::integral_constant<int, 2 * RT>{});
   });
 }
 
@@ -934,23 +991,16 @@ static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& 
                        AT ? static_cast<int64_t>(rank) : 1, accumulate);
     return launch_status("tiny_outer_kernel");
   }
-  const int parts = outer_parts(sg.tokens, sg.nslots, width, rank);
+  const int parts = outer_parts(sg.tokens, sg.nslots, width);
   const int64_t per = rank * width, stride = per * sg.nslots;
-  auto go = [&](auto rt, auto pc) {
-    constexpr int RT = decltype(rt)::value, PC = decltype(pc)::value;
-    const dim3 grid(static_cast<unsigned>(cdiv(width, 64 * PC)), static_cast<unsigned>(sg.nslots), parts);
-    hipLaunchKernelGGL((outer_kernel<T, RT, PC, AT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx, H,
-                       sg, static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg,
-                       stride, accumulate);
+  const int rc = with_tile(sg, rank, [&](auto, auto rt) {
+    constexpr int RT = decltype(rt)::value;
+    const dim3 grid(static_cast<unsigned>(cdiv(width, 64 * kOuterCols)), static_cast<unsigned>(sg.nslots), parts);
+    hipLaunchKernelGGL((outer_kernel<T, RT, AT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx, H, sg,
+                       static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg, stride,
+                       accumulate);
     return launch_status("outer_kernel");
-  };
-  const std::integral_constant<int, 1> one;
-  const std::integral_constant<int, 2> two;
-  const std::integral_constant<int, 4> four;
-  const std::integral_constant<int, 8> eight;
-  const bool wide = outer_cols(width, sg.nslots, rank) == 8;
-  const int rc = rank > 32 ? go(four, four)
-                 : rank > 16 ? (wide ? go(two, eight) : go(two, four)) : (wide ? go(one, eight) : go(one, four));
+  });
   if (rc || parts == 1) return rc;
   const dim3 jg(static_cast<unsigned>(cdiv(per, 256)), static_cast<unsigned>(sg.nslots));
   hipLaunchKernelGGL((join_parts_kernel<AT>), jg, dim3(256), 0, st, parts_ws, parts, stride, sg,

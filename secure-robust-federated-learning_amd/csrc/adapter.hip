@@ -312,8 +312,10 @@ static int tile_count(const Segs& sg) {
 // rows at a time: every 16 bytes a cache line of its own.  So operands that more
 // than one lane group shares, or whose rows are memory's rows, are read in
 // whole lines, brought into fragments once a workgroup, and put into LDS as
-// pieces (row, c) of 8 inner values, piece c at c * (ROWS + 1) + row: 16 rows of
-// a fragment read, and the neighbours that write, fall into different banks.
+// pieces (row, c) of 8 inner values.  Their places let any 8 neighbouring lanes of
+// a read (rows n, or n * PERM + a for n = 0..15) and of a write fall into
+// different banks: row r at (r % PERM) * kStep + r / PERM, with kStep and the
+// distance of pieces padded for that.
 //
 // TR false: element (row, inner) at src[row * ld + inner].  TR true: at
 // src[inner * ld + row]; a thread then loads 4 rows of 8 inner values and turns
@@ -322,10 +324,12 @@ static int tile_count(const Segs& sg) {
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-template <typename T, typename S, int ROWS, int PIECES, bool TR>
+template <typename T, typename S, int ROWS, int PIECES, bool TR, int PERM>
 struct Stage {
   using F = Frag<T, S>;
-  static constexpr int kPlane = PIECES * (ROWS + 1);
+  static constexpr int kStep = PERM == 8 ? ROWS / 8 + 1 : PERM == 4 ? ROWS / 4 + 2 : 0;
+  static constexpr int kPiece = PERM == 1 ? ROWS + 1 : PERM * kStep + (TR ? 4 : 1);
+  static constexpr int kPlane = PIECES * kPiece;
   static constexpr int kBytes = kPlane * kPlanes<F> * 16;
   static constexpr int kUnits = TR ? ROWS / 4 * PIECES : ROWS * PIECES;
   static constexpr int kEach = (kUnits + kThreads - 1) / kThreads;
@@ -363,6 +367,9 @@ struct Stage {
     return min(q * kThreads + static_cast<int>(threadIdx.x), kUnits - 1);
   }
 
+  static __device__ __forceinline__ int place(int row, int c) {
+    return c * kPiece + (PERM == 1 ? row : row % PERM * kStep + row / PERM);
+  }
   __device__ __forceinline__ int64_t turn_at(int k, int row) const { return min(k, inner - 1) * ld + row; }
   __device__ __forceinline__ int64_t line_at(int u) const { return min(u / PIECES, rows - 1) * ld + u % PIECES * 8; }
 
@@ -385,7 +392,7 @@ struct Stage {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               put_elem<T, S>(f, e, c * 8 + e < inner ? r[q].turn[e].get(a) : static_cast<S>(0.f));
-            put_frag(lds, kPlane, c * (ROWS + 1) + row + a, f);
+            put_frag(lds, kPlane, place(row + a, c), f);
           }
       } else {
         const int k = u % PIECES * 8;
@@ -397,14 +404,14 @@ struct Stage {
 #pragma unroll
           for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, k + e < inner ? r[q].line.get(e) : static_cast<S>(0.f));
         }
-        if (in) put_frag(lds, kPlane, u % PIECES * (ROWS + 1) + u / PIECES, f);
+        if (in) put_frag(lds, kPlane, place(u / PIECES, u % PIECES), f);
       }
     }
   }
 
   static __device__ __forceinline__ F get(const u32x4* lds, int row, int c) {
     F f;
-    get_frag(f, lds, kPlane, c * (ROWS + 1) + row);
+    get_frag(f, lds, kPlane, place(row, c));
     return f;
   }
 };
@@ -425,8 +432,8 @@ __global__ void __launch_bounds__(kThreads)
     shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, Segs sg, int width,
                   int parts, int part, int rank, float* __restrict__ H) {
   constexpr int KB = kShrinkCols<T, RT, NT>, PIECES = KB / 8;
-  using SX = Stage<T, T, 16 * NT, PIECES, false>;
-  using SW = Stage<T, W, 16 * RT, PIECES, AT>;
+  using SX = Stage<T, T, 16 * NT, PIECES, false, 1>;
+  using SW = Stage<T, W, 16 * RT, PIECES, AT, AT ? 4 : 1>;
   __shared__ u32x4 lds[(SX::kBytes + SW::kBytes) / 16];
   u32x4* const ldw_ = lds + SX::kBytes / 16;
   const int tile = static_cast<int>(blockIdx.x) / parts, pt = static_cast<int>(blockIdx.x) % parts;
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(kThreads)
                   int64_t ldw, Segs sg, int width, int blocks, int span, int rank, float scale, T* out, int64_t ldo,
                   float* __restrict__ Hsum) {
   constexpr int COLS = kExpandCols<NT>, PC = NT == 1 ? 4 : 8, RK = (RP + 3) / 4;
-  using SW = Stage<T, W, COLS, RP, !AT>;                 // RP pieces of 8 ranks
+  using SW = Stage<T, W, COLS, RP, !AT, PC>;                 // RP pieces of 8 ranks
   __shared__ u32x4 lds[SW::kBytes / 16];
   const int tile = static_cast<int>(blockIdx.x) / blocks, block = static_cast<int>(blockIdx.x) % blocks;
   const Tile tl = find_tile<16 * NT>(sg, tile);
@@ -666,7 +673,7 @@ template <typename T, int RT, bool AT>
 __global__ void __launch_bounds__(kThreads)
     outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
                  float scale, float* __restrict__ G, int64_t ldg, int64_t part_stride, int accumulate) {
-  using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true>;
+  using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true, 4>;
   constexpr int PC = kOuterCols;
   __shared__ u32x4 lds[SH::kBytes / 16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;

@@ -21,13 +21,14 @@ struct Tokens {
   int64_t tokens, vocab, dim;
 };
 
-// row of the (nslots * vocab, dim) table that token t reads, -1 for none
-__device__ __forceinline__ int64_t token_row(const Tokens& k, int64_t t, int& slot, int64_t& id) {
+// row of the (nslots * vocab, dim) table that token t reads, -1 for none; one
+// caller a token counts its fault
+__device__ __forceinline__ int64_t token_row(const Tokens& k, int64_t t, int& slot, int64_t& id, bool count) {
   slot = token_slot(k.offsets, k.slots, k.nseg, k.nslots, t);
   id = k.ids[t];
   if (slot < 0) return -1;
   if (id < 0 || id >= k.vocab) {
-    count_row_fault();
+    if (count) count_row_fault();
     return -1;
   }
   return slot * k.vocab + id;
@@ -43,61 +44,145 @@ __device__ __forceinline__ float scaled(float v, float scale) {
   return r;
 }
 
-template <typename W, typename T>
+// 8 consecutive values of a row at any alignment of their type (the hardware's
+// global accesses take it)
+typedef u32x4 __attribute__((aligned(2))) any_u32x4;
+
+template <typename S>
+struct Row8 {
+  u32x4 v[sizeof(S) / 2];
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(S) == 4) {
+      const unsigned word = v[e / 4][e % 4];
+      return __builtin_bit_cast(float, word);
+    } else {
+      return to_f32(__builtin_bit_cast(S, static_cast<unsigned short>(v[0][e / 2] >> (e % 2 * 16))));
+    }
+  }
+};
+
+template <typename S>
+__device__ __forceinline__ Row8<S> load8(const S* p) {
+  Row8<S> r;
+#pragma unroll
+  for (int b = 0; b < static_cast<int>(sizeof(S) / 2); ++b) r.v[b] = reinterpret_cast<const any_u32x4*>(p)[b];
+  return r;
+}
+
+template <typename S>
+__device__ __forceinline__ void store8(S* p, const float (&x)[8]) {
+  union {
+    u32x4 v[sizeof(S) / 2];
+    S s[8];
+  } q;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q.s[e] = from_f32<S>(x[e]);
+#pragma unroll
+  for (int b = 0; b < static_cast<int>(sizeof(S) / 2); ++b) reinterpret_cast<any_u32x4*>(p)[b] = q.v[b];
+}
+
+// Lookup: LANES lanes a token, 8 values a lane and step.  Bound by memory (a
+// read of the row, a write of the output); 16 lanes keep every lane busy at odd
+// widths, 64 spread few tokens over more waves.
+template <typename W, typename T, int LANES>
 __global__ void __launch_bounds__(256) embed_kernel(const W* __restrict__ table, int64_t ldt, Tokens k, float scale,
                                                     T* __restrict__ out, int64_t ldo) {
-  const int64_t t = blockIdx.x;
-  __shared__ int64_t src;
-  if (threadIdx.x == 0) {
-    int slot;
-    int64_t id;
-    src = token_row(k, t, slot, id) < 0 ? -1 : slot * ldt + id * k.dim;
+  const int64_t t = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+  if (t >= k.tokens) return;
+  const int first = static_cast<int>(threadIdx.x % LANES) * 8;
+  int slot;
+  int64_t id;
+  const bool none = token_row(k, t, slot, id, first == 0) < 0;
+  const int dim = static_cast<int>(k.dim);
+  const W* src = table + (none ? 0 : slot * ldt + id * k.dim);
+  T* dst = out + t * ldo;
+#pragma unroll 4
+  for (int j = first; j < dim; j += LANES * 8) {
+    if (j + 8 <= dim) {
+      const Row8<W> r = load8(src + j);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = none ? 0.f : scaled(r.get(e), scale);
+      store8(dst + j, x);
+    } else {
+      for (int e = j; e < dim; ++e) dst[e] = from_f32<T>(none ? 0.f : scaled(to_f32(src[e]), scale));
+    }
   }
-  __syncthreads();
-  const int64_t from = src;
-  for (int64_t j = threadIdx.x; j < k.dim; j += 256)
-    out[t * ldo + j] = from_f32<T>(from < 0 ? 0.f : scaled(to_f32(table[from + j]), scale));
 }
 
 // ---------------------------------------------------------------------------
 // Sort: key = row << 32 | position, unique, so any correct sort is stable.
-// Tokens without a row get the largest row and stay behind.
+// Tokens without a row get the largest row and stay behind.  Tiles of 4096 are
+// sorted in LDS: runs of 1, 2, 4, ... merged by rank, an element moving to its
+// place in its own run plus the count of smaller ones in the partner run, each
+// thread's 4 searches in step.  The same launch clears the gradient with the
+// workgroups behind the sorting ones: the sort hides behind that write.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 4096;
 constexpr int kSortThreads = 1024;
+constexpr int kOwn = kTile / kSortThreads;
 constexpr unsigned kNoRow = 0xffffffffu;
 
-__global__ void __launch_bounds__(kSortThreads) sort_tiles_kernel(Tokens k, int64_t padding,
-                                                                  uint64_t* __restrict__ keys) {
+struct Clear {
+  float* grad;
+  int64_t ldg, per;          // floats of a slot
+  int blocks;                // workgroups a slot
+};
+
+__device__ __forceinline__ void clear_rows(const Clear& z, int64_t block) {
+  float* g = z.grad + block / z.blocks * z.ldg;
+  const int64_t stride = static_cast<int64_t>(z.blocks) * kSortThreads * 4;
+  for (int64_t i = (block % z.blocks * kSortThreads + threadIdx.x) * 4; i < z.per; i += stride) {
+    if (i + 4 <= z.per) {
+      reinterpret_cast<any_u32x4*>(g + i)[0] = u32x4{0, 0, 0, 0};
+    } else {
+      for (int64_t e = i; e < z.per; ++e) g[e] = 0.f;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_tiles_kernel(Tokens k, int64_t padding, int tiles,
+                                                                  uint64_t* __restrict__ keys, Clear clear) {
   __shared__ uint64_t buf[2][kTile];
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    clear_rows(clear, static_cast<int64_t>(blockIdx.x) - tiles);
+    return;
+  }
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTile;
   const int n = static_cast<int>(min(static_cast<int64_t>(kTile), k.tokens - t0));
-  for (int i = threadIdx.x; i < kTile; i += kSortThreads) {
+  int top = 1;
+  while (top < n) top <<= 1;
+  for (int i = threadIdx.x; i < top; i += kSortThreads) {
     unsigned row = kNoRow;
     if (i < n) {
       int slot;
       int64_t id;
-      const int64_t r = token_row(k, t0 + i, slot, id);
+      const int64_t r = token_row(k, t0 + i, slot, id, true);
       if (r >= 0 && id != padding) row = static_cast<unsigned>(r);
     }
     buf[0][i] = static_cast<uint64_t>(row) << 32 | static_cast<uint32_t>(t0 + i);
   }
   __syncthreads();
-  // runs of 1, 2, 4, ... merged by rank: an element moves to its place in its
-  // own run plus the count of smaller ones in the partner run
   int cur = 0;
-  int top = 1;
-  while (top < n) top <<= 1;
   for (int len = 1; len < top; len <<= 1) {
-    for (int i = threadIdx.x; i < top; i += kSortThreads) {
-      const uint64_t key = buf[cur][i];
-      const int mine = i & ~(len - 1), other = mine ^ len, base = mine & ~(2 * len - 1);
-      int lo = 0, hi = len;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (buf[cur][other + mid] < key) lo = mid + 1; else hi = mid;
-      }
-      buf[cur ^ 1][base + (i - mine) + lo] = key;
+    uint64_t key[kOwn];
+    int at[kOwn], to[kOwn];
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+      const int i = min(q * kSortThreads + static_cast<int>(threadIdx.x), top - 1);
+      key[q] = buf[cur][i];
+      at[q] = (i & ~(len - 1)) ^ len;                                  // the partner run
+      to[q] = (i & ~(2 * len - 1)) + (i & (len - 1)) - at[q];          // place, less what `at` counts from
+    }
+    // lower bound in len sorted keys: halve, then one last comparison
+    for (int step = len >> 1; step > 0; step >>= 1)
+#pragma unroll
+      for (int q = 0; q < kOwn; ++q)
+        if (buf[cur][at[q] + step - 1] < key[q]) at[q] += step;
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+      if (buf[cur][at[q]] < key[q]) ++at[q];
+      if (q * kSortThreads + static_cast<int>(threadIdx.x) < top) buf[cur ^ 1][at[q] + to[q]] = key[q];
     }
     cur ^= 1;
     __syncthreads();
@@ -106,89 +191,201 @@ __global__ void __launch_bounds__(kSortThreads) sort_tiles_kernel(Tokens k, int6
 }
 
 // Sorted tiles into one sorted list: an element's place is its place in its own
-// tile plus the count of smaller elements of every other tile.
-__global__ void __launch_bounds__(256) merge_tiles_kernel(const uint64_t* __restrict__ keys, int64_t tokens,
+// tile plus the count of smaller elements of every other tile, 4 searches in step.
+__global__ void __launch_bounds__(256) merge_tiles_kernel(const uint64_t* __restrict__ keys, int tokens, int tiles,
                                                           uint64_t* __restrict__ sorted) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int i = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
   if (i >= tokens) return;
   const uint64_t key = keys[i];
-  const int64_t mine = i / kTile;
-  int64_t place = i - mine * kTile;
-  for (int64_t q = 0; q * kTile < tokens; ++q) {
-    if (q == mine) continue;
-    int64_t lo = q * kTile, hi = min(lo + kTile, tokens);
-    const int64_t from = lo;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  const int mine = i / kTile;
+  int place = i - mine * kTile;
+  for (int q0 = 0; q0 < tiles; q0 += 4) {
+    int64_t at[4], from[4];
+    int n[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      from[q] = at[q] = static_cast<int64_t>(min(q0 + q, tiles - 1)) * kTile;
+      const bool search = q0 + q < tiles && q0 + q != mine;
+      n[q] = search ? static_cast<int>(min(static_cast<int64_t>(kTile), tokens - at[q])) : 0;
     }
-    place += lo - from;
+    // keys at and beyond n count as larger
+    for (int step = kTile / 2; step > 0; step >>= 1)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t probe = at[q] + step - 1;
+        const bool in = probe - from[q] < n[q];
+        if (in && keys[in ? probe : from[q]] < key) at[q] += step;
+      }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool in = at[q] - from[q] < n[q];
+      if (in && keys[in ? at[q] : from[q]] < key) ++at[q];
+      place += static_cast<int>(at[q] - from[q]);
+    }
   }
   sorted[place] = key;
 }
 
-__global__ void __launch_bounds__(256) fill_rows_kernel(float* __restrict__ grad, int64_t ldg, int64_t per_slot) {
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  float* g = grad + blockIdx.y * ldg;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < per_slot; i += stride) g[i] = 0.f;
-}
-
 // ---------------------------------------------------------------------------
-// Sum: a workgroup takes kWindow sorted positions of 256 columns.  Runs that
-// lie inside the window go to their row; a run that the window shares with the
-// one before (head) or after (tail) leaves a partial sum.  The window where
-// such a run starts then adds up the partials in order.
+// Sum: a wave takes 32 sorted positions of 512 columns, 8 rows' loads in flight.
+// Runs that lie inside the window go to their row; a run that the window shares
+// with the one before (head) or after (tail) leaves a partial sum.  The window
+// where such a run starts then adds up the partials in order.
 // ---------------------------------------------------------------------------
 constexpr int kWindow = 32;
+constexpr int kBatch = 8;
+constexpr int kCols = 512;
 
 __device__ __forceinline__ unsigned row_at(const uint64_t* __restrict__ sorted, int64_t i) {
   return static_cast<unsigned>(sorted[i] >> 32);
 }
 
-__device__ __forceinline__ void put(float* grad, int64_t ldg, const Tokens& k, unsigned row, int64_t j, float v,
-                                    int accumulate) {
-  const int64_t slot = row / k.vocab, id = row % k.vocab;
-  float* g = grad + slot * ldg + id * k.dim + j;
-  *g = accumulate ? *g + v : v;
-}
+struct Grad {
+  float* grad;
+  int64_t ldg;
+  float scale;
+  int accumulate;
+};
 
-template <typename T>
-__global__ void __launch_bounds__(256) sum_windows_kernel(const T* __restrict__ dout, int64_t lddo, Tokens k,
-                                                          const uint64_t* __restrict__ sorted, float scale,
-                                                          float* __restrict__ grad, int64_t ldg, int accumulate,
-                                                          float* __restrict__ head, float* __restrict__ tail) {
-  const int64_t w = blockIdx.x, from = w * kWindow, to = min(from + kWindow, k.tokens);
-  const int64_t j = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x;
-  if (j >= k.dim) return;
-  float a = 0.f;
-  bool shared_front = from > 0 && row_at(sorted, from - 1) == row_at(sorted, from);
-  for (int64_t i = from; i < to; ++i) {
-    const unsigned row = row_at(sorted, i);
-    if (row == kNoRow) break;
-    a += to_f32(dout[static_cast<int64_t>(static_cast<uint32_t>(sorted[i])) * lddo + j]);
-    if (i + 1 < to && row_at(sorted, i + 1) == row) continue;
-    const bool shared_back = i + 1 == to && to < k.tokens && row_at(sorted, to) == row;
-    if (shared_front) head[w * k.dim + j] = a;            // also when it goes on behind the window
-    else if (shared_back) tail[w * k.dim + j] = a;
-    else put(grad, ldg, k, row, j, a * scale, accumulate);
-    shared_front = false;
-    a = 0.f;
+__device__ __forceinline__ void put_cols(float* p, const float (&a)[8], int valid) {
+  if (valid >= 8) {
+    store8(p, a);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < valid) p[e] = a[e];
   }
 }
 
-__global__ void __launch_bounds__(256) join_windows_kernel(Tokens k, const uint64_t* __restrict__ sorted, float scale,
-                                                           float* __restrict__ grad, int64_t ldg, int accumulate,
-                                                           const float* __restrict__ head,
+__device__ __forceinline__ void put_row(const Grad& o, const Tokens& k, unsigned row, int j, const float (&a)[8],
+                                        int valid) {
+  const unsigned vocab = static_cast<unsigned>(k.vocab), slot = row / vocab, id = row % vocab;
+  float* g = o.grad + static_cast<int64_t>(slot) * o.ldg + static_cast<int64_t>(id) * k.dim + j;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = a[e] * o.scale;
+  if (o.accumulate)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < valid) v[e] += g[e];
+  put_cols(g, v, valid);
+}
+
+// WIDE: rows of at least 8 values, read 8 at a time; lanes whose 8 would pass the
+// end of the row read the last 8 and use their upper ones
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) sum_windows_kernel(const T* __restrict__ dout, int64_t lddo, Tokens k,
+                                                          const uint64_t* __restrict__ sorted, Grad o, int chunks,
+                                                          int64_t units, float* __restrict__ head,
+                                                          float* __restrict__ tail) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= units) return;
+  const int64_t w = unit / chunks, from = w * kWindow, to = min(from + kWindow, k.tokens);
+  const int dim = static_cast<int>(k.dim);
+  const int j = static_cast<int>(unit % chunks) * kCols + static_cast<int>(threadIdx.x & 63) * 8;
+  if (j >= dim) return;
+  const int valid = min(8, dim - j), shift = WIDE ? 8 - valid : 0;
+  float a[8] = {};
+  unsigned row = row_at(sorted, from);
+  bool shared_front = from > 0 && row_at(sorted, from - 1) == row;
+  for (int64_t i0 = from; i0 < to && row != kNoRow; i0 += kBatch) {
+    Row8<T> r[kBatch];
+    uint64_t key[kBatch + 1];
+#pragma unroll
+    for (int q = 0; q <= kBatch; ++q) key[q] = i0 + q < k.tokens ? sorted[i0 + q] : ~uint64_t{0};
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const T* p = dout + static_cast<int64_t>(static_cast<uint32_t>(key[i0 + q < to ? q : 0])) * lddo + j;
+      if constexpr (WIDE) {
+        r[q] = load8(p - shift);
+      } else {
+        union {
+          Row8<T> r;
+          T t[8];
+        } u = {};
+        for (int e = 0; e < valid; ++e) u.t[e] = p[e];
+        r[q] = u.r;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (i0 + q >= to || row == kNoRow) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] += r[q].get(e);
+      const unsigned next = static_cast<unsigned>(key[q + 1] >> 32);
+      const bool end = i0 + q + 1 == to;
+      if (next == row && !end) continue;
+      if (WIDE && shift != 0) {                              // the upper values belong to this lane's columns
+        float u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          u[e] = 0.f;
+#pragma unroll
+          for (int f = e; f < 8; ++f)
+            if (f - e == shift) u[e] = a[f];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = u[e];
+      }
+      if (shared_front) put_cols(head + w * k.dim + j, a, valid);    // also when it goes on behind the window
+      else if (end && next == row && to < k.tokens) put_cols(tail + w * k.dim + j, a, valid);
+      else put_row(o, k, row, j, a, valid);
+      shared_front = false;
+      row = next;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = 0.f;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) join_windows_kernel(Tokens k, const uint64_t* __restrict__ sorted, Grad o,
+                                                           int chunks, int64_t units, const float* __restrict__ head,
                                                            const float* __restrict__ tail) {
-  const int64_t w = blockIdx.x, from = w * kWindow, to = from + kWindow;
-  const int64_t j = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x;
-  if (j >= k.dim || to >= k.tokens) return;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= units) return;
+  const int64_t w = unit / chunks, from = w * kWindow, to = from + kWindow;
+  const int dim = static_cast<int>(k.dim);
+  const int j = static_cast<int>(unit % chunks) * kCols + static_cast<int>(threadIdx.x & 63) * 8;
+  if (to >= k.tokens) return;
   const unsigned row = row_at(sorted, to - 1);
   if (row == kNoRow || row_at(sorted, to) != row) return;                       // nothing goes on
   if (from > 0 && row_at(sorted, from - 1) == row) return;                      // started further to the front
-  float a = tail[w * k.dim + j];
-  for (int64_t v = w + 1; v * kWindow < k.tokens && row_at(sorted, v * kWindow) == row; ++v) a += head[v * k.dim + j];
-  put(grad, ldg, k, row, j, a * scale, accumulate);
+  // how many windows the run goes on for, 64 at a time
+  int64_t last = w + 1;
+  for (const int64_t windows = (k.tokens + kWindow - 1) / kWindow;; last += 64) {
+    const int64_t v = last + static_cast<int64_t>(threadIdx.x & 63);
+    const unsigned long long on = __ballot(v < windows && row_at(sorted, min(v, windows - 1) * kWindow) == row);
+    if (~on != 0) {
+      last += __ffsll(~on) - 1;
+      break;
+    }
+  }
+  if (j >= dim) return;                                                        // every lane was needed above
+  const int valid = min(8, dim - j);
+  float a[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a[e] = e < valid ? tail[w * k.dim + j + e] : 0.f;
+  for (int64_t v0 = w + 1; v0 < last; v0 += kBatch) {
+    float h[kBatch][8];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const float* p = head + min(v0 + q, last - 1) * k.dim + j;
+      if (valid == 8) {
+        const Row8<float> r = load8(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[q][e] = r.get(e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[q][e] = e < valid ? p[e] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (v0 + q < last)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] += h[q][e];
+  }
+  put_row(o, k, row, j, a, valid);
 }
 
 static int check_table(const Tokens& k, int64_t ldt) {
@@ -245,10 +442,15 @@ extern "C" int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const i
     return with_type(odtype, [&](auto t) {
       using W = decltype(w);
       using T = decltype(t);
-      hipLaunchKernelGGL((embed_kernel<W, T>), dim3(static_cast<unsigned>(tokens)), dim3(256), 0,
-                         static_cast<hipStream_t>(stream), static_cast<const W*>(table), ldt, k, scale,
-                         static_cast<T*>(out), ldo);
-      return launch_status("embed_kernel");
+      // 16 lanes a token unless that leaves the card less than 4 waves a compute unit
+      const bool few = tokens * 16 < 64 * 1024;
+      const dim3 grid(static_cast<unsigned>(cdiv(tokens * (few ? 64 : 16), 256)));
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const W*>(table),
+                           ldt, k, scale, static_cast<T*>(out), ldo);
+        return launch_status("embed_kernel");
+      };
+      return few ? go(embed_kernel<W, T, 64>) : go(embed_kernel<W, T, 16>);
     });
   });
 }
@@ -282,37 +484,39 @@ extern "C" int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, con
   uint64_t* sorted = reinterpret_cast<uint64_t*>(base + p.sorted);
   float* head = reinterpret_cast<float*>(base + p.head);
   float* tail = reinterpret_cast<float*>(base + p.tail);
+  const int tiles = static_cast<int>(cdiv(tokens, kTile));
+  Clear clear{grad, ldg, vocab * dim, 0};
   if (!accumulate) {
-    const int64_t per = vocab * dim;
-    const unsigned gx = static_cast<unsigned>(std::min<int64_t>(cdiv(per, 256), 4096));
-    for (int32_t c = 0; c < nslots; c += 65535) {
-      const unsigned gy = static_cast<unsigned>(std::min<int32_t>(nslots - c, 65535));
-      hipLaunchKernelGGL(fill_rows_kernel, dim3(gx, gy), dim3(256), 0, st, grad + c * ldg, ldg, per);
-      if (int rc = launch_status("fill_rows_kernel")) return rc;
-    }
+    // enough workgroups to fill the card, each with 4 stores a thread or more
+    const int64_t most = cdiv(clear.per, kSortThreads * 16);
+    clear.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, cdiv(4096, nslots))));
   }
-  if (tokens == 0) return SRA_OK;
-  const int64_t tiles = cdiv(tokens, kTile);
-  hipLaunchKernelGGL(sort_tiles_kernel, dim3(static_cast<unsigned>(tiles)), dim3(kSortThreads), 0, st, k, padding,
-                     tiles > 1 ? keys : sorted);
+  if (tiles == 0 && accumulate) return SRA_OK;
+  const int64_t blocks = tiles + static_cast<int64_t>(clear.blocks) * nslots;
+  SRA_REQUIRE(blocks < (int64_t{1} << 31), SRA_ERR_UNSUPPORTED, "%d slots are too many", nslots);
+  hipLaunchKernelGGL(sort_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), 0, st, k, padding,
+                     tiles, tiles > 1 ? keys : sorted, clear);
   if (int rc = launch_status("sort_tiles_kernel")) return rc;
+  if (tokens == 0) return SRA_OK;
   if (tiles > 1) {
     hipLaunchKernelGGL(merge_tiles_kernel, dim3(static_cast<unsigned>(cdiv(tokens, 256))), dim3(256), 0, st, keys,
-                       tokens, sorted);
+                       static_cast<int>(tokens), tiles, sorted);
     if (int rc = launch_status("merge_tiles_kernel")) return rc;
   }
-  const dim3 grid(static_cast<unsigned>(cdiv(tokens, kWindow)), static_cast<unsigned>(cdiv(dim, 256)));
+  const int chunks = static_cast<int>(cdiv(dim, kCols));
+  const int64_t units = cdiv(tokens, kWindow) * chunks;
+  const dim3 grid(static_cast<unsigned>(cdiv(units, 4)));
+  const Grad o{grad, ldg, scale, accumulate};
   const int rc = with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((sum_windows_kernel<T>), grid, dim3(256), 0, st, static_cast<const T*>(dout), lddo, k, sorted,
-                       scale, grad, ldg, accumulate, head, tail);
-    return launch_status("sum_windows_kernel");
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, static_cast<const T*>(dout), lddo, k, sorted, o, chunks, units,
+                         head, tail);
+      return launch_status("sum_windows_kernel");
+    };
+    return dim >= 8 ? go(sum_windows_kernel<T, true>) : go(sum_windows_kernel<T, false>);
   });
-  if (rc) return rc;
-  if (tokens > kWindow) {
-    hipLaunchKernelGGL(join_windows_kernel, grid, dim3(256), 0, st, k, sorted, scale, grad, ldg, accumulate, head,
-                       tail);
-    return launch_status("join_windows_kernel");
-  }
-  return SRA_OK;
+  if (rc || tokens <= kWindow) return rc;
+  hipLaunchKernelGGL(join_windows_kernel, grid, dim3(256), 0, st, k, sorted, o, chunks, units, head, tail);
+  return launch_status("join_windows_kernel");
 }

@@ -550,11 +550,10 @@ int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t*
  *   grad_i = grad_logp * (1[i = target] - p_i) - grad_entropy * p_i (log p_i + entropy)
  * (no logp part for an ignored target; grad_entropy may be NULL), which reads
  * the logits from memory once for both. */
-int sra_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top, size_t* bytes);
 int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
                        int64_t vocab, int64_t ignore, int32_t top, float* logp, float* entropy, float* lse,
                        float* top_logp, int64_t* top_ids, const float* grad_logp, const float* grad_entropy,
-                       void* grad, int64_t ldg, void* ws, size_t ws_bytes, void* stream);
+                       void* grad, int64_t ldg, void* stream);
 
 /* The same gradient from a forward pass's lse and entropy (entropy is needed
  * with grad_entropy only). */

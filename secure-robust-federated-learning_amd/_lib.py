@@ -136,9 +136,8 @@ _SIGS = {
     "sra_embed_grad_workspace_bytes": [_i64, _i64, ctypes.POINTER(_sz)],
     "sra_embed_grad": [_ptr, _i64, _i32, _ptr, _ptr, _ptr, _i32, _i64, _i32, _i64, _i64, ctypes.c_float, _i64,
                        _ptr, _i64, _i32, _ptr, _sz, _ptr],
-    "sra_token_logprobs_workspace_bytes": [_i64, _i64, _i32, ctypes.POINTER(_sz)],
     "sra_token_logprobs": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
-                           _ptr, _ptr, _i64, _ptr, _sz, _ptr],
+                           _ptr, _ptr, _i64, _ptr],
     "sra_token_logprobs_grad": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64,
                                 _ptr],
 }

@@ -227,17 +227,25 @@ __global__ void __launch_bounds__(256) merge_tiles_kernel(const uint64_t* __rest
 }
 
 // ---------------------------------------------------------------------------
-// Sum: a wave takes 32 sorted positions of 512 columns, 8 rows' loads in flight.
+// Sum: a wave takes a window of sorted positions and 512 columns, 8 rows' loads in
+// flight.
 // Runs that lie inside the window go to their row; a run that the window shares
 // with the one before (head) or after (tail) leaves a partial sum.  The window
 // where such a run starts then adds up the partials in order.
 // ---------------------------------------------------------------------------
-constexpr int kWindow = 32;
 constexpr int kBatch = 8;
 constexpr int kCols = 512;
 
 __device__ __forceinline__ unsigned row_at(const uint64_t* __restrict__ sorted, int64_t i) {
   return static_cast<unsigned>(sorted[i] >> 32);
+}
+
+// Positions a window: 32 (a partial sum for 32 rows read), fewer where the waves
+// would not fill the card.
+static int window_of(int64_t tokens, int64_t dim) {
+  int w = 32;
+  while (w > 8 && cdiv(tokens, w) * cdiv(dim, kCols) < 4096) w /= 2;
+  return w;
 }
 
 struct Grad {
@@ -275,12 +283,12 @@ __device__ __forceinline__ void put_row(const Grad& o, const Tokens& k, unsigned
 // end of the row read the last 8 and use their upper ones
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) sum_windows_kernel(const T* __restrict__ dout, int64_t lddo, Tokens k,
-                                                          const uint64_t* __restrict__ sorted, Grad o, int chunks,
-                                                          int64_t units, float* __restrict__ head,
+                                                          const uint64_t* __restrict__ sorted, Grad o, int window,
+                                                          int chunks, int64_t units, float* __restrict__ head,
                                                           float* __restrict__ tail) {
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit >= units) return;
-  const int64_t w = unit / chunks, from = w * kWindow, to = min(from + kWindow, k.tokens);
+  const int64_t w = unit / chunks, from = w * window, to = min(from + window, k.tokens);
   const int dim = static_cast<int>(k.dim);
   const int j = static_cast<int>(unit % chunks) * kCols + static_cast<int>(threadIdx.x & 63) * 8;
   if (j >= dim) return;
@@ -339,11 +347,11 @@ __global__ void __launch_bounds__(256) sum_windows_kernel(const T* __restrict__ 
 }
 
 __global__ void __launch_bounds__(256) join_windows_kernel(Tokens k, const uint64_t* __restrict__ sorted, Grad o,
-                                                           int chunks, int64_t units, const float* __restrict__ head,
+                                                           int window, int chunks, int64_t units, const float* __restrict__ head,
                                                            const float* __restrict__ tail) {
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit >= units) return;
-  const int64_t w = unit / chunks, from = w * kWindow, to = from + kWindow;
+  const int64_t w = unit / chunks, from = w * window, to = from + window;
   const int dim = static_cast<int>(k.dim);
   const int j = static_cast<int>(unit % chunks) * kCols + static_cast<int>(threadIdx.x & 63) * 8;
   if (to >= k.tokens) return;
@@ -352,9 +360,9 @@ __global__ void __launch_bounds__(256) join_windows_kernel(Tokens k, const uint6
   if (from > 0 && row_at(sorted, from - 1) == row) return;                      // started further to the front
   // how many windows the run goes on for, 64 at a time
   int64_t last = w + 1;
-  for (const int64_t windows = (k.tokens + kWindow - 1) / kWindow;; last += 64) {
+  for (const int64_t windows = (k.tokens + window - 1) / window;; last += 64) {
     const int64_t v = last + static_cast<int64_t>(threadIdx.x & 63);
-    const unsigned long long on = __ballot(v < windows && row_at(sorted, min(v, windows - 1) * kWindow) == row);
+    const unsigned long long on = __ballot(v < windows && row_at(sorted, min(v, windows - 1) * window) == row);
     if (~on != 0) {
       last += __ffsll(~on) - 1;
       break;
@@ -408,7 +416,7 @@ struct GradPlan {
 
 static GradPlan grad_plan(int64_t tokens, int64_t dim) {
   GradPlan p{};
-  const int64_t windows = cdiv(tokens, kWindow);
+  const int64_t windows = cdiv(tokens, window_of(tokens, dim));
   p.keys = 0;
   p.sorted = p.keys + static_cast<size_t>(tokens) * 8;
   p.head = p.sorted + static_cast<size_t>(tokens) * 8;
@@ -487,9 +495,10 @@ extern "C" int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, con
   const int tiles = static_cast<int>(cdiv(tokens, kTile));
   Clear clear{grad, ldg, vocab * dim, 0};
   if (!accumulate) {
-    // enough workgroups to fill the card, each with 4 stores a thread or more
-    const int64_t most = cdiv(clear.per, kSortThreads * 16);
-    clear.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, cdiv(4096, nslots))));
+    // one store a thread (983 MB: 156 us, against 172 us with 15 stores a thread),
+    // more only where that would be too many workgroups for a launch
+    const int64_t most = cdiv(clear.per, kSortThreads * 4);
+    clear.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (int64_t{1} << 30) / nslots)));
   }
   if (tiles == 0 && accumulate) return SRA_OK;
   const int64_t blocks = tiles + static_cast<int64_t>(clear.blocks) * nslots;
@@ -504,19 +513,21 @@ extern "C" int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, con
     if (int rc = launch_status("merge_tiles_kernel")) return rc;
   }
   const int chunks = static_cast<int>(cdiv(dim, kCols));
-  const int64_t units = cdiv(tokens, kWindow) * chunks;
+  const int window = window_of(tokens, dim);
+  const int64_t units = cdiv(tokens, window) * chunks;
   const dim3 grid(static_cast<unsigned>(cdiv(units, 4)));
   const Grad o{grad, ldg, scale, accumulate};
   const int rc = with_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, static_cast<const T*>(dout), lddo, k, sorted, o, chunks, units,
-                         head, tail);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, static_cast<const T*>(dout), lddo, k, sorted, o, window,
+                         chunks, units, head, tail);
       return launch_status("sum_windows_kernel");
     };
     return dim >= 8 ? go(sum_windows_kernel<T, true>) : go(sum_windows_kernel<T, false>);
   });
-  if (rc || tokens <= kWindow) return rc;
-  hipLaunchKernelGGL(join_windows_kernel, grid, dim3(256), 0, st, k, sorted, o, chunks, units, head, tail);
+  if (rc || tokens <= window) return rc;
+  hipLaunchKernelGGL(join_windows_kernel, grid, dim3(256), 0, st, k, sorted, o, window, chunks, units, head,
+                     tail);
   return launch_status("join_windows_kernel");
 }

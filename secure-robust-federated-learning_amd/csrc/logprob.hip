@@ -555,18 +555,11 @@ static int with_type(int32_t dtype, F&& f) {
 
 using namespace sra;
 
-extern "C" int sra_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top, size_t* bytes) {
-  SRA_REQUIRE(bytes != nullptr, SRA_ERR_ARG, "null bytes pointer");
-  SRA_REQUIRE(rows >= 0 && vocab >= 1 && top >= 0, SRA_ERR_SHAPE, "rows, vocab and top must not be negative");
-  *bytes = 16;
-  return SRA_OK;
-}
-
 extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
                                   int64_t rows, int64_t vocab, int64_t ignore, int32_t top, float* logp,
                                   float* entropy, float* lse, float* top_logp, int64_t* top_ids,
                                   const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
-                                  void* ws, size_t ws_bytes, void* stream) {
+                                  void* stream) {
   if (int rc = check_logits(logits, ldl, dtype, targets, rows, vocab)) return rc;
   SRA_REQUIRE(top >= 0 && top <= vocab, SRA_ERR_ARG, "top must be in [0, vocab], got %d", top);
   SRA_REQUIRE(top <= SRA_TOKEN_MAX_TOP, SRA_ERR_UNSUPPORTED, "top %d is above %d", top, SRA_TOKEN_MAX_TOP);
@@ -576,10 +569,6 @@ extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype
   SRA_REQUIRE(grad == nullptr || grad_logp != nullptr, SRA_ERR_ARG, "the gradient needs grad_logp");
   if (grad != nullptr)
     if (int rc = check_grad(logits, ldl, grad, ldg, rows, vocab, dtype)) return rc;
-  size_t need = 0;
-  if (int rc = sra_token_logprobs_workspace_bytes(rows, vocab, top, &need)) return rc;
-  SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "token_logprobs workspace: need %zu bytes, got %zu",
-              need, ws_bytes);
   if (rows == 0) return SRA_OK;
   const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, top, logp, entropy, lse, top_logp, top_ids,
                grad_logp, grad_entropy, ldg};

@@ -26,11 +26,12 @@ through torch's caching allocator.  There is no CPU path.
 """
 from __future__ import annotations
 
+import functools
 from collections import namedtuple
 
 import torch
 
-from . import _lib, engine
+from . import _lib
 
 MAX_RANK = 64
 MAX_TOP = 32
@@ -40,7 +41,8 @@ TokenLogprobs = namedtuple("TokenLogprobs", "logp entropy lse top_logp top_ids")
 
 
 # ---------------------------------------------------------------------------
-# argument checks
+# argument checks: the usual tensors (contiguous, of the expected shape) pass on
+# the first line of each, the small calls are bound by this code
 # ---------------------------------------------------------------------------
 def _device_tensor(name, t, device=None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -51,52 +53,53 @@ def _device_tensor(name, t, device=None):
 
 
 def _float_code(name, t):
-    if t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    return _DTYPES[t.dtype]
+    return code
 
 
-def _rows(name, t, shape=None, dtype=None, device=None, out=False):
-    """A matrix the kernels can walk as row * stride + column.  Inputs whose
-    columns are strided or whose rows overlap are copied; outputs are refused."""
+def _check(name, t, shape, dtype, device):
     _device_tensor(name, t, device)
-    if t.dim() != 2:
-        raise ValueError("%s must be a matrix, got shape %s" % (name, tuple(t.shape)))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    r, c = t.shape
-    if (c > 1 and t.stride(1) != 1) or (r > 1 and t.stride(0) < c):
+
+
+def _rows(name, t, shape, dtype, device, out=False):
+    """A matrix the kernels can walk as row * stride + column, and that stride.
+    Inputs whose columns are strided or whose rows overlap are copied; outputs are
+    refused."""
+    _check(name, t, shape, dtype, device)
+    r, c = shape
+    if t.is_contiguous():
+        return t, c
+    s0, s1 = t.stride()
+    if (c > 1 and s1 != 1) or (r > 1 and s0 < c):
         if out:
             raise ValueError("%s needs unit column stride and rows that do not overlap" % name)
-        t = t.contiguous()
-    return t, (t.stride(0) if r > 1 else c)
+        return t.contiguous(), c
+    return t, (s0 if r > 1 else c)
 
 
 def _slot_rows(name, t, shape, device, dtype=None, out=False):
-    """(n, *matrix) whose matrices are contiguous: slot stride only."""
-    _device_tensor(name, t, device)
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    n, per = t.shape[0], t.shape[1] * t.shape[2]
-    inner = (t.shape[1] == 1 or t.stride(1) == t.shape[2]) and (t.shape[2] == 1 or t.stride(2) == 1)
-    if not inner or (n > 1 and t.stride(0) < per):
+    """(n, *matrix) whose matrices are contiguous, and the slot stride."""
+    _check(name, t, shape, dtype, device)
+    n, a, b = shape
+    if t.is_contiguous():
+        return t, a * b
+    s0, s1, s2 = t.stride()
+    if (a > 1 and s1 != b) or (b > 1 and s2 != 1) or (n > 1 and s0 < a * b):
         if out:
             raise ValueError("%s needs contiguous slots that do not overlap" % name)
-        t = t.contiguous()
-    return t, (t.stride(0) if n > 1 else per)
+        return t.contiguous(), a * b
+    return t, (s0 if n > 1 else a * b)
 
 
 def _vector(name, t, n, dtype, device):
-    _device_tensor(name, t, device)
-    if t.dtype != dtype:
-        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    if tuple(t.shape) != (n,):
-        raise ValueError("%s must have shape (%d,), got %s" % (name, n, tuple(t.shape)))
-    return t.contiguous()
+    _check(name, t, (n,), dtype, device)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _segments(offsets, slots, device):
@@ -105,19 +108,31 @@ def _segments(offsets, slots, device):
     _device_tensor("slots", slots, device)
     if slots.dim() != 1:
         raise ValueError("slots must be a vector, got shape %s" % (tuple(slots.shape),))
-    slots = _vector("slots", slots, slots.shape[0], torch.int32, device)
-    offsets = _vector("offsets", offsets, slots.shape[0] + 1, torch.int64, device)
-    return offsets, slots, slots.shape[0]
+    n = slots.shape[0]
+    return (_vector("offsets", offsets, n + 1, torch.int64, device), _vector("slots", slots, n, torch.int32, device), n)
 
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(device, name, *args):
     """One library call on the device's current stream (the last argument)."""
-    with torch.cuda.device(device):
-        _lib.call(name, *args, engine._stream_ptr(device))
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _raw_stream(index))
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(name, *args):
+    """A workspace size: a function of the sizes alone."""
+    return _lib.query_bytes(name, *args)
 
 
 # ---------------------------------------------------------------------------
@@ -141,7 +156,7 @@ def _adapter_args(x, A, B, offsets, slots):
         raise TypeError("A and B must both be float32 or %s, got %s and %s" % (x.dtype, A.dtype, B.dtype))
     A, lda = _slot_rows("A", A, (n, r, K), x.device)
     B, ldb = _slot_rows("B", B, (n, M, r), x.device)
-    x, ldx = _rows("x", x)
+    x, ldx = _rows("x", x, (T, K), x.dtype, x.device)
     offsets, slots, S = _segments(offsets, slots, x.device)
     head = (x.data_ptr(), ldx, A.data_ptr(), lda, B.data_ptr(), ldb, offsets.data_ptr(), slots.data_ptr(), S, T, n, K,
             M, r)
@@ -150,8 +165,8 @@ def _adapter_args(x, A, B, offsets, slots):
 
 
 def _adapter_workspace(T, S, n, K, M, r, device):
-    nb = _lib.query_bytes("sra_adapter_workspace_bytes", T, S, n, K, M, r)
-    return engine._workspace(nb, device), nb
+    nb = _bytes("sra_adapter_workspace_bytes", T, S, n, K, M, r)
+    return torch.empty(nb, dtype=torch.uint8, device=device), nb
 
 
 def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=False):
@@ -168,9 +183,11 @@ def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=Fal
     ldbase = M
     if base is not None:
         base, ldbase = _rows("base", base, (T, M), x.dtype, dev)
+    ldo = M
     if out is None:
         out = torch.empty((T, M), dtype=x.dtype, device=dev)
-    out, ldo = _rows("out", out, (T, M), x.dtype, dev, out=True)
+    else:
+        out, ldo = _rows("out", out, (T, M), x.dtype, dev, out=True)
     H = torch.empty((T, r), dtype=torch.float32, device=dev) if hidden else None
     ws, nb = _adapter_workspace(T, slots.shape[0], n, K, M, r, dev)
     _call(dev, "sra_adapter_apply", _ptr(base), ldbase, *head, float(scale), dtype, wdtype, out.data_ptr(), ldo,
@@ -285,8 +302,8 @@ def embed_grad(grad_out, ids, grad, offsets=None, slots=None, scale=1.0, padding
         pad = int(padding_idx)
         if not 0 <= pad < V:
             raise ValueError("padding_idx must be in [0, %d), got %d" % (V, pad))
-    nb = _lib.query_bytes("sra_embed_grad_workspace_bytes", T, E)
-    ws = engine._workspace(nb, dev)
+    nb = _bytes("sra_embed_grad_workspace_bytes", T, E)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     _call(dev, "sra_embed_grad", dy.data_ptr(), lddy, code, ids.data_ptr(), _ptr(off), _ptr(sl), S, T, n, V, E,
           float(scale), pad, full.data_ptr(), ld, int(bool(accumulate)), ws.data_ptr(), nb)
     return grad
@@ -300,7 +317,7 @@ def _logits(logits, targets):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be (rows, vocab), got %s" % (tuple(logits.shape),))
     code = _float_code("logits", logits)
-    logits, ldl = _rows("logits", logits)
+    logits, ldl = _rows("logits", logits, logits.shape, logits.dtype, logits.device)
     targets = _vector("targets", targets, logits.shape[0], torch.int64, logits.device)
     return logits, ldl, code, targets
 
@@ -316,10 +333,11 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
     if top > MAX_TOP:
         raise NotImplementedError("top %d is above %d" % (top, MAX_TOP))
 
-    def new(*shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=dev)
-
-    res = TokenLogprobs(new(R), new(R) if entropy else None, new(R), new(R, top), new(R, top, dtype=torch.int64))
+    # logp, lse and the alternatives come as views of one buffer
+    f = torch.empty((2 + bool(entropy) + top) * R, dtype=torch.float32, device=dev)
+    rows = f[:(2 + bool(entropy)) * R].view(2 + bool(entropy), R).unbind(0)
+    res = TokenLogprobs(rows[0], rows[2] if entropy else None, rows[1], f[(2 + bool(entropy)) * R:].view(R, top),
+                        torch.empty((R, top), dtype=torch.int64, device=dev))
     grad, ldg = None, 0
     if grad_logp is not None:
         grad_logp = _vector("grad_logp", grad_logp, R, torch.float32, dev)
@@ -327,13 +345,12 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
             grad_entropy = _vector("grad_entropy", grad_entropy, R, torch.float32, dev)
         if out is src and logits is not src:
             raise ValueError("out can be the logits only where they have unit column stride")
-        grad, ldg = _rows("out", new(R, V, dtype=logits.dtype) if out is None else out, (R, V), logits.dtype, dev,
-                          out=True)
-    nb = _lib.query_bytes("sra_token_logprobs_workspace_bytes", R, V, top)
-    ws = engine._workspace(nb, dev)
+        if out is None:
+            out = torch.empty((R, V), dtype=logits.dtype, device=dev)
+        grad, ldg = _rows("out", out, (R, V), logits.dtype, dev, out=True)
     _call(dev, "sra_token_logprobs", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V, int(ignore_index), top,
           res.logp.data_ptr(), _ptr(res.entropy), res.lse.data_ptr(), res.top_logp.data_ptr(), res.top_ids.data_ptr(),
-          _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad), ldg, ws.data_ptr(), nb)
+          _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad), ldg)
     return res, grad
 
 

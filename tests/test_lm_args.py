@@ -98,11 +98,11 @@ def test_embed_grad_refuses(kw, exc, match):
     (dict(top=101, vocab=100), ValueError, "top"), (dict(top_ids=None), ValueError, "top"),
     (dict(grad_logp=None), ValueError, "grad_logp"), (dict(ldg=99), ValueError, "stride"),
     (dict(ldg=101), ValueError, "one buffer"), (dict(dtype=9), ValueError, "dtype"),
-    (dict(logits=ctypes.c_void_p(4097)), ValueError, "aligned"), (dict(ws=None), ValueError, "workspace"),
+    (dict(logits=ctypes.c_void_p(4097)), ValueError, "aligned"),
 ])
 def test_token_logprobs_refuses(kw, exc, match):
     a = dict(logits=P, ldl=100, dtype=1, targets=P, rows=4, vocab=100, ignore=-100, top=2, logp=P, entropy=P, lse=P,
-             top_logp=P, top_ids=P, grad_logp=P, grad_entropy=None, grad=P, ldg=100, ws=P, ws_bytes=BIG)
+             top_logp=P, top_ids=P, grad_logp=P, grad_entropy=None, grad=P, ldg=100)
     a.update(kw)
     with pytest.raises(exc, match=match):
         _lib.call("sra_token_logprobs", *a.values(), None)
@@ -136,5 +136,5 @@ def test_python_entry_points_need_device_tensors():
 def test_zero_rows_and_tokens_need_no_launch():
     _lib.call("sra_adapter_apply", *adapter_args(tokens=0))
     _lib.call("sra_token_logprobs", None, 100, 1, None, 0, 100, -100, 0, None, None, None, None, None, None, None, None,
-              0, P, 64, None)
+              0, None)
     _lib.call("sra_embed", P, 8, 0, None, None, None, 0, 0, 1, 4, 2, 1.0, None, 2, 0, None)

@@ -751,33 +751,42 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int a = 0; a < PC; ++a) {
         if (a >= valid) continue;
-        float* p = gc + (AT && last ? static_cast<int64_t>(j + a) * rank + i : static_cast<int64_t>(i) * width + j + a);
+        float* p = gc + (AT ? static_cast<int64_t>(j + a) * rank + i : static_cast<int64_t>(i) * width + j + a);
         const float v = f * acc[r][a][q];
         *p = add ? *p + v : v;
       }
     }
 }
 
-// G_c = scale * sum of the parts, in order
-template <bool AT>
+// G_c = scale * sum of the parts, in order; 4 values a thread
 __global__ void __launch_bounds__(256)
-    join_parts_kernel(const float* __restrict__ P, int parts, int64_t part_stride, Segs sg, int width, int rank,
-                      float scale, float* __restrict__ G, int64_t ldg, int accumulate) {
+    join_parts_kernel(const float* __restrict__ P, int parts, int64_t part_stride, Segs sg, int64_t per, float scale,
+                      float* __restrict__ G, int64_t ldg, int accumulate) {
   const int c = blockIdx.y;
-  const int64_t per = static_cast<int64_t>(rank) * width;
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t q = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (q >= per) return;
   if (accumulate) {
     bool any = false;
     for (int s = 0; s < sg.nseg; ++s) any |= sg.slots[s] == c && seg_start(sg, s + 2) > seg_start(sg, s + 1);
     if (!any) return;
   }
-  const int64_t i = AT ? q % rank : q / width, j = AT ? q / rank : q % width;
-  const float* p = P + c * per + i * width + j;
-  float a = p[0];
-  for (int z = 1; z < parts; ++z) a += p[z * part_stride];
+  const float* p = P + c * per;
+  float a[4] = {};
+  for (int z = 0; z < parts; ++z) {
+    Raw4<float> r = load_at<float, 4>(p + z * part_stride, q, per);
+    settle(r, q, per);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += r.get(e);
+  }
   float* o = G + c * ldg + q;
-  *o = accumulate ? *o + scale * a : scale * a;
+  const int valid = static_cast<int>(min(per - q, int64_t{4}));
+  Raw4<float> v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float old = accumulate && e < valid ? o[e] : 0.f;
+    v.set(e, old + scale * a[e]);
+  }
+  store_n(o, v, valid);
 }
 
 // ---------------------------------------------------------------------------
@@ -892,13 +901,14 @@ static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
   return p;
 }
 
-// Parts of a client's tokens that outer sums apart: two workgroups a compute
-// unit, each with at least 2 stages of tokens.
+// Parts of a client's tokens that outer sums apart: four workgroups a compute
+// unit, each with at least 2 stages of tokens on average (clients with more hold
+// the launch up less, the join costs a pass over the parts).
 static int outer_parts(int64_t tokens, int nslots, int64_t width) {
   const int64_t blocks = cdiv(width, 64 * kOuterCols) * nslots;
   const int64_t stages = cdiv(tokens, kOuterTokens * static_cast<int64_t>(nslots));
   int p = 1;
-  while (p < kMaxParts && blocks * p < 512 && stages >= 4 * p) p *= 2;
+  while (p < kMaxParts && blocks * p < 1024 && stages >= 2 * p) p *= 2;
   return p;
 }
 
@@ -1009,9 +1019,9 @@ static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& 
     return launch_status("outer_kernel");
   });
   if (rc || parts == 1) return rc;
-  const dim3 jg(static_cast<unsigned>(cdiv(per, 256)), static_cast<unsigned>(sg.nslots));
-  hipLaunchKernelGGL((join_parts_kernel<AT>), jg, dim3(256), 0, st, parts_ws, parts, stride, sg,
-                     static_cast<int>(width), rank, scale, G, ldg, accumulate);
+  const dim3 jg(static_cast<unsigned>(cdiv(per, 1024)), static_cast<unsigned>(sg.nslots));
+  hipLaunchKernelGGL(join_parts_kernel, jg, dim3(256), 0, st, parts_ws, parts, stride, sg, per, scale, G, ldg,
+                     accumulate);
   return launch_status("join_parts_kernel");
 }
 

@@ -35,6 +35,22 @@ unsigned int adapter_row_faults(bool reset) { return tu_row_faults(reset); }
 // ---------------------------------------------------------------------------
 // 8 values a lane, and their products
 // ---------------------------------------------------------------------------
+// Two values in a word, rounded to nearest even, and back
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, pair));
+}
+template <typename T>
+__device__ __forceinline__ f32x2 unpack2(unsigned w) {
+  if constexpr (std::is_same_v<T, __bf16>)
+    return f32x2{__builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)};
+  else
+    return f32x2{to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(w))),
+                 to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(w >> 16)))};
+}
+
 // N stored values as they came, in words: a load's registers stay untouched, and
 // unwaited for, until get takes a value out of them.
 template <typename S, int N>
@@ -42,15 +58,24 @@ struct RawN {
   static constexpr int kWords = N * static_cast<int>(sizeof(S)) / 4;
   unsigned w[kWords];
   __device__ __forceinline__ S get(int e) const {
-    if constexpr (sizeof(S) == 4) return __builtin_bit_cast(S, w[e]);
-    else return __builtin_bit_cast(S, static_cast<unsigned short>(w[e / 2] >> (e % 2 * 16)));
-  }
-  __device__ __forceinline__ void set(int e, S v) {
     if constexpr (sizeof(S) == 4) {
-      w[e] = __builtin_bit_cast(unsigned, v);
+      const unsigned v = w[e];
+      return __builtin_bit_cast(S, v);
     } else {
-      const unsigned b = __builtin_bit_cast(unsigned short, v);
-      w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | b << 16 : (w[e / 2] & 0xffff0000u) | b;
+      return __builtin_bit_cast(S, static_cast<unsigned short>(w[e / 2] >> (e % 2 * 16)));
+    }
+  }
+  // values e and e + 1, e even
+  __device__ __forceinline__ f32x2 get2(int e) const {
+    if constexpr (sizeof(S) == 4) return f32x2{get(e), get(e + 1)};
+    else return unpack2<S>(w[e / 2]);
+  }
+  __device__ __forceinline__ void set2(int e, float a, float b) {
+    if constexpr (sizeof(S) == 4) {
+      w[e] = __builtin_bit_cast(unsigned, a);
+      w[e + 1] = __builtin_bit_cast(unsigned, b);
+    } else {
+      w[e / 2] = pack2<S>(a, b);
     }
   }
 };
@@ -98,27 +123,35 @@ __device__ __forceinline__ void settle(RawN<S, N>& r, int64_t o, int64_t n) {
   if (__ballot(d > 0 && d < N) == 0) return;
   const int by = d > 0 ? static_cast<int>(d) : 0;
   constexpr int kWords = RawN<S, N>::kWords, kPer = 4 / sizeof(S);
-  auto words_down = [&](auto step) {                     // by a constant: registers have no address
+  // by constants and masks: registers have no address to choose by
+  auto words_down = [&](auto step) {
     constexpr int kStep = decltype(step)::value;
     if constexpr (kStep < kWords) {
-      const bool on = (by & (kStep * kPer)) != 0;
+      const unsigned on = (by & (kStep * kPer)) != 0 ? 0xffffffffu : 0u;
 #pragma unroll
-      for (int e = 0; e + kStep < kWords; ++e) {
-        const unsigned from = r.w[e + kStep], at = r.w[e];
-        r.w[e] = on ? from : at;
-      }
+      for (int e = 0; e + kStep < kWords; ++e) r.w[e] = (r.w[e + kStep] & on) | (r.w[e] & ~on);
     }
   };
   words_down(std::integral_constant<int, 4>{});
   words_down(std::integral_constant<int, 2>{});
   words_down(std::integral_constant<int, 1>{});
   if constexpr (sizeof(S) == 2) {
-    const bool on = (by & 1) != 0;
+    const unsigned on = (by & 1) != 0 ? 0xffffffffu : 0u;
 #pragma unroll
     for (int e = 0; e < kWords; ++e) {
-      const unsigned next = e + 1 < kWords ? r.w[e + 1] : 0u, at = r.w[e];
-      r.w[e] = on ? at >> 16 | next << 16 : at;
+      const unsigned next = e + 1 < kWords ? r.w[e + 1] : 0u;
+      r.w[e] = ((r.w[e] >> 16 | next << 16) & on) | (r.w[e] & ~on);
     }
+  }
+}
+
+// values from `valid` on become zero
+template <typename S, int N>
+__device__ __forceinline__ void cut(RawN<S, N>& r, int valid) {
+#pragma unroll
+  for (int b = 0; b < RawN<S, N>::kWords; ++b) {
+    if constexpr (sizeof(S) == 4) r.w[b] &= b < valid ? 0xffffffffu : 0u;
+    else r.w[b] &= 2 * b + 1 < valid ? 0xffffffffu : 2 * b < valid ? 0xffffu : 0u;
   }
 }
 
@@ -139,42 +172,58 @@ __device__ __forceinline__ void store_n(S* p, const RawN<S, N>& r, int valid) {
   }
 }
 
+// 8 operand values a lane: bf16 terms, two values a word, or floats
 template <int N>
 struct Terms {
-  bf16x8 t[N];
+  unsigned t[N][4];
+  __device__ __forceinline__ bf16x8 term(int i) const {
+    return __builtin_bit_cast(bf16x8, u32x4{t[i][0], t[i][1], t[i][2], t[i][3]});
+  }
 };
 struct Floats {
   float v[8];
 };
-
-// nearest bf16 and the rest
-__device__ __forceinline__ void split_into(Terms<2>& f, int e, float x) {
-  const __bf16 hi = static_cast<__bf16>(x);
-  const float h = static_cast<float>(hi);
-  f.t[0][e] = hi;
-  f.t[1][e] = static_cast<__bf16>(x - h);
-}
 
 // the operand that T's matrix units take for stored values S
 template <typename T, typename S>
 using Frag = std::conditional_t<std::is_same_v<T, float>, Floats,
                                 Terms<std::is_same_v<S, __bf16> ? 1 : 2>>;
 
-template <typename T, typename S>
-__device__ __forceinline__ void put_elem(Frag<T, S>& f, int e, S x) {
-  if constexpr (std::is_same_v<T, float>) f.v[e] = x;
-  else if constexpr (std::is_same_v<S, __bf16>) f.t[0][e] = x;
-  else split_into(f, e, static_cast<float>(x));
+// values e and e + 1, e even: the nearest bf16 and the rest
+__device__ __forceinline__ void put2(Terms<2>& f, int e, f32x2 x) {
+  const unsigned hi = pack2<__bf16>(x[0], x[1]);
+  const f32x2 h = unpack2<__bf16>(hi);
+  f.t[0][e / 2] = hi;
+  f.t[1][e / 2] = pack2<__bf16>(x[0] - h[0], x[1] - h[1]);
+}
+__device__ __forceinline__ void put2(Floats& f, int e, f32x2 x) {
+  f.v[e] = x[0];
+  f.v[e + 1] = x[1];
 }
 
 template <typename T, typename S>
 __device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
   Frag<T, S> f;
   if constexpr (std::is_same_v<S, __bf16>) {
-    f.t[0] = __builtin_bit_cast(bf16x8, u32x4{r.w[0], r.w[1], r.w[2], r.w[3]});
+#pragma unroll
+    for (int b = 0; b < 4; ++b) f.t[0][b] = r.w[b];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, r.get(e));
+    for (int e = 0; e < 8; e += 2) put2(f, e, r.get2(e));
+  }
+  return f;
+}
+
+// column a of 8 rows
+template <typename T, typename S, int N>
+__device__ __forceinline__ Frag<T, S> column_of(const RawN<S, N> (&r)[8], int a) {
+  Frag<T, S> f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    if constexpr (std::is_same_v<S, __bf16>)
+      f.t[0][e / 2] = __builtin_amdgcn_perm(r[e + 1].w[a / 2], r[e].w[a / 2], a % 2 ? 0x07060302u : 0x05040100u);
+    else
+      put2(f, e, f32x2{to_f32(r[e].get(a)), to_f32(r[e + 1].get(a))});
   }
   return f;
 }
@@ -183,26 +232,32 @@ __device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
 template <int N>
 __device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Terms<N>& f) {
 #pragma unroll
-  for (int p = 0; p < N; ++p) lds[p * plane + at] = __builtin_bit_cast(u32x4, f.t[p]);
+  for (int p = 0; p < N; ++p) lds[p * plane + at] = u32x4{f.t[p][0], f.t[p][1], f.t[p][2], f.t[p][3]};
 }
 __device__ __forceinline__ void put_frag(u32x4* lds, int plane, int at, const Floats& f) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    u32x4 v;
-    __builtin_memcpy(&v, f.v + 4 * p, 16);
-    lds[p * plane + at] = v;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = f.v[4 * p + e];
+    lds[p * plane + at] = __builtin_bit_cast(u32x4, v);
   }
 }
 template <int N>
 __device__ __forceinline__ void get_frag(Terms<N>& f, const u32x4* lds, int plane, int at) {
 #pragma unroll
-  for (int p = 0; p < N; ++p) f.t[p] = __builtin_bit_cast(bf16x8, lds[p * plane + at]);
+  for (int p = 0; p < N; ++p) {
+    const u32x4 v = lds[p * plane + at];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) f.t[p][b] = v[b];
+  }
 }
 __device__ __forceinline__ void get_frag(Floats& f, const u32x4* lds, int plane, int at) {
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    const u32x4 v = lds[p * plane + at];
-    __builtin_memcpy(f.v + 4 * p, &v, 16);
+    const f32x4 v = __builtin_bit_cast(f32x4, lds[p * plane + at]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.v[4 * p + e] = v[e];
   }
 }
 template <typename F>
@@ -214,7 +269,7 @@ __device__ __forceinline__ void mma(f32x4& acc, const Terms<N>& a, const Terms<M
   for (int i = N - 1; i >= 0; --i)
 #pragma unroll
     for (int j = M - 1; j >= 0; --j)
-      if (i + j < 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t[i], b.t[j], acc, 0, 0, 0);
+      if (i + j < 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.term(i), b.term(j), acc, 0, 0, 0);
 }
 
 __device__ __forceinline__ void mma(f32x4& acc, const Floats& a, const Floats& b) {
@@ -333,11 +388,7 @@ struct Stage {
   static constexpr int kBytes = kPlane * kPlanes<F> * 16;
   static constexpr int kUnits = TR ? ROWS / 4 * PIECES : ROWS * PIECES;
   static constexpr int kEach = (kUnits + kThreads - 1) / kThreads;
-  union Unit {
-    Raw8<S> line;
-    Raw4<S> turn[TR ? 8 : 1];
-  };
-  Unit r[kEach];
+  RawN<S, TR ? 4 : 8> r[kEach][TR ? 8 : 1];                // a line, or 8 to turn
   int64_t ld, total;
   int rows, inner;
 
@@ -355,9 +406,9 @@ struct Stage {
       if constexpr (TR) {
         const int row = u % (ROWS / 4) * 4, k = u / (ROWS / 4) * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[q].turn[e] = load_at<S, 4>(src, turn_at(k + e, row), total);
+        for (int e = 0; e < 8; ++e) r[q][e] = load_at<S, 4>(src, turn_at(k + e, row), total);
       } else {
-        r[q].line = load_at<S, 8>(src, line_at(u), total);
+        r[q][0] = load_at<S, 8>(src, line_at(u), total);
       }
     }
   }
@@ -376,6 +427,7 @@ struct Stage {
   __device__ __forceinline__ void put(u32x4* lds) {
     // whether any load of this stage ended before its place
     const bool near = TR ? turn_at(8 * PIECES, ROWS) > total : (rows - 1) * ld + 8 * PIECES > total;
+    const bool partial = inner < 8 * PIECES;
 #pragma unroll
     for (int q = 0; q < kEach; ++q) {
       const bool in = kUnits % kThreads == 0 || q * kThreads + static_cast<int>(threadIdx.x) < kUnits;
@@ -384,27 +436,29 @@ struct Stage {
         const int row = u % (ROWS / 4) * 4, c = u / (ROWS / 4);
         if (near)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) settle(r[q].turn[e], turn_at(c * 8 + e, row), total);
-        if (in)
+          for (int e = 0; e < 8; ++e) settle(r[q][e], turn_at(c * 8 + e, row), total);
+        if constexpr (std::is_same_v<T, float>) {
+          if (in)
 #pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            F f;
+            for (int a = 0; a < 4; ++a) {
+              F f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              put_elem<T, S>(f, e, c * 8 + e < inner ? r[q].turn[e].get(a) : static_cast<S>(0.f));
-            put_frag(lds, kPlane, place(row + a, c), f);
-          }
+              for (int e = 0; e < 8; ++e) f.v[e] = c * 8 + e < inner ? r[q][e].get(a) : 0.f;
+              put_frag(lds, kPlane, place(row + a, c), f);
+            }
+        } else {
+          if (partial)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) cut(r[q][e], c * 8 + e < inner ? 4 : 0);
+          if (in)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) put_frag(lds, kPlane, place(row + a, c), column_of<T, S>(r[q], a));
+        }
       } else {
         const int k = u % PIECES * 8;
-        F f;
-        if (inner >= 8 * PIECES) {
-          f = frag_of<T, S>(r[q].line);
-        } else {
-          if (near) settle(r[q].line, line_at(u), total);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) put_elem<T, S>(f, e, k + e < inner ? r[q].line.get(e) : static_cast<S>(0.f));
-        }
-        if (in) put_frag(lds, kPlane, place(u / PIECES, u % PIECES), f);
+        if (near) settle(r[q][0], line_at(u), total);
+        if (partial) cut(r[q][0], inner - k);
+        if (in) put_frag(lds, kPlane, place(u / PIECES, u % PIECES), frag_of<T, S>(r[q][0]));
       }
     }
   }
@@ -580,7 +634,7 @@ __global__ void __launch_bounds__(kThreads)
           if (i + e < rank) Hsum[at + i + e] = h[e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) put_elem<T, float>(fh[b], e, h[e] * scale);
+    for (int e = 0; e < 8; e += 2) put2(fh[b], e, f32x2{h[e] * scale, h[e + 1] * scale});
   }
   const int row = (NT == 1 ? wave * 64 : 0) + n * PC;    // this lane's columns of a stage
   auto base_at = [&](int q, int j0) { return (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j0 + row; };
@@ -616,7 +670,10 @@ __global__ void __launch_bounds__(kThreads)
       if (base != nullptr && j0 + COLS > c1) settle(r[q], base_at(q, j0), ball);
       if (t < tl.n) {
 #pragma unroll
-        for (int a = 0; a < PC; ++a) r[q].set(a, from_f32<T>(to_f32(r[q].get(a)) + acc[a][q]));
+        for (int a = 0; a < PC; a += 2) {
+          const f32x2 v = r[q].get2(a);
+          r[q].set2(a, v[0] + acc[a][q], v[1] + acc[a + 1][q]);
+        }
         store_n(out + (tl.t0 + t) * ldo + j, r[q], j0 + COLS <= c1 ? PC : c1 - j);
       }
       r[q] = nxt[q];
@@ -723,9 +780,7 @@ __global__ void __launch_bounds__(kThreads)
             if (b * 32 + g * 8 + e >= left_now) q[b][e] = RawN<T, PC>{};
         Frag<T, T> fx[PC];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int a = 0; a < PC; ++a) put_elem<T, T>(fx[a], e, q[b][e].get(a));
+        for (int a = 0; a < PC; ++a) fx[a] = column_of<T, T>(q[b], a);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);
@@ -782,10 +837,9 @@ __global__ void __launch_bounds__(256)
   const int valid = static_cast<int>(min(per - q, int64_t{4}));
   Raw4<float> v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float old = accumulate && e < valid ? o[e] : 0.f;
-    v.set(e, old + scale * a[e]);
-  }
+  for (int e = 0; e < 4; e += 2)
+    v.set2(e, (accumulate && e < valid ? o[e] : 0.f) + scale * a[e],
+           (accumulate && e + 1 < valid ? o[e + 1] : 0.f) + scale * a[e + 1]);
   store_n(o, v, valid);
 }
 

@@ -476,7 +476,8 @@ int sra_bulyan_dba_f32(const float* X, int64_t n, int64_t d, int64_t ldx, int32_
  * to, or -1 for none.  Two segments may share a slot.  Tokens that no segment
  * covers have no slot.  A slot outside [-1, nslots) or a token id outside the
  * vocabulary counts as none and is reported by sra_row_fault_count; offsets
- * outside [0, tokens] are clamped. */
+ * outside [0, tokens] are clamped.  A call that would need a launch of 2^32
+ * threads or more is refused. */
 typedef enum { SRA_F32 = 0, SRA_BF16 = 1, SRA_F16 = 2 } sra_dtype;
 
 /* Largest adapter rank, and most alternatives of sra_token_logprobs. */
@@ -504,7 +505,8 @@ int sra_adapter_apply(const void* base, int64_t ldbase, const void* x, int64_t l
  *   z_t = B_c' dout_t,   dx_t = dxbase_t + scale * A_c' z_t
  *   dA_c = scale * sum_t z_t x_t',   dB_c = scale * sum_t dout_t h_t'
  * dx (dtype), dA (float32, slot stride ldda) and dB (float32, slot stride
- * lddb) are each optional (NULL); dxbase may be NULL (zeros) or equal dx.
+ * lddb) are each optional (NULL); dxbase may be NULL (zeros) or equal dx, which
+ * must be neither dout nor x.
  * Every slot of dA and dB is written, zeros where a slot has no token;
  * accumulate != 0 adds to them instead.  No atomics: results do not depend on
  * the order in which workgroups run. */

@@ -683,12 +683,14 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---------------------------------------------------------------------------
 // outer: G_c[i, j] = scale * sum over the tokens t of slot c of H[t, i] x[t, j].
-// The inner index is the token.  A workgroup takes one slot, 64 PC columns and
-// every gridDim.z-th stage of 128 of its tokens; H is staged for the 4 waves,
-// which own 16 PC columns each: a lane loads PC columns of 8 tokens, the
-// operands of PC products with columns n * PC + a.  With one part the sums go to
-// G ([i][j], or [j][i] with AT), else each part's to its own copy (slot stride
-// rank * width) for join_parts.
+// The inner index is the token.  A workgroup takes one slot, every gridDim.z-th
+// stage of 128 of its tokens, staged as H for its 4 waves, and 16 PC columns a
+// wave: a lane loads PC columns of 8 tokens, the operands of PC products with
+// columns n * PC + a.  With SPLIT the waves share 16 PC columns, take a quarter
+// of each stage's tokens and add their sums in a fixed order: four times the
+// workgroups where there are few.  With one part the sums go to G ([i][j], or
+// [j][i] with AT), else each part's to its own copy (slot stride rank * width)
+// for join_parts.
 // ---------------------------------------------------------------------------
 constexpr int kOuterTokens = 128;
 constexpr int kOuterCols = 4;
@@ -726,27 +728,28 @@ struct SlotStages {
   }
 };
 
-template <typename T, int RT, bool AT>
+template <typename T, int RT, bool AT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads)
     outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
                  float scale, float* __restrict__ G, int64_t ldg, int64_t part_stride, int accumulate) {
   using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true, 4>;
-  constexpr int PC = kOuterCols;
-  __shared__ u32x4 lds[SH::kBytes / 16];
+  constexpr int PC = kOuterCols, NB = SPLIT ? 1 : kOuterTokens / 32, kSums = SPLIT ? 2 * RT * PC * 64 : 0;
+  __shared__ u32x4 lds[SH::kBytes / 16 > kSums ? SH::kBytes / 16 : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
-  const int c = blockIdx.y, j = ((static_cast<int>(blockIdx.x) * 4 + wave) * 16 + n) * PC;
+  const int c = blockIdx.y, block = static_cast<int>(blockIdx.x);
+  const int j = ((SPLIT ? block : block * 4 + wave) * 16 + n) * PC, k0 = SPLIT ? wave * 32 : 0;
   const int valid = max(0, min(PC, width - j));
-  const bool whole = (static_cast<int>(blockIdx.x) + 1) * 64 * PC <= width;
+  const bool whole = (block + 1) * (SPLIT ? 16 : 64) * PC <= width;
   const int64_t xall = (sg.tokens - 1) * ldx + width;      // elements of x
   const int turns = static_cast<int>(gridDim.z);
   f32x4 acc[RT][PC] = {};
   SlotStages it{sg, c, static_cast<int>(blockIdx.z), turns};
   SH sh;
-  RawN<T, PC> q[kOuterTokens / 32][8];
+  RawN<T, PC> q[NB][8];
   int t, left;
   bool more = it.next(t, left);
-  auto x_at = [&](int b, int e) { return static_cast<int64_t>(t + min(b * 32 + g * 8 + e, left - 1)) * ldx + j; };
+  auto x_at = [&](int b, int e) { return static_cast<int64_t>(t + min(k0 + b * 32 + g * 8 + e, left - 1)) * ldx + j; };
   auto fetch = [&](int b) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[b][e] = load_at<T, PC>(x, x_at(b, e), xall);
@@ -757,8 +760,8 @@ __global__ void __launch_bounds__(kThreads)
   if (more) {
     fetch_h();
 #pragma unroll
-    for (int b = 0; b < kOuterTokens / 32; ++b)
-      if (b * 32 < left) fetch(b);
+    for (int b = 0; b < NB; ++b)
+      if (k0 + b * 32 < left) fetch(b);
   }
   while (more) {
     __syncthreads();
@@ -768,28 +771,43 @@ __global__ void __launch_bounds__(kThreads)
     more = it.next(t, left);
     if (more) fetch_h();
 #pragma unroll
-    for (int b = 0; b < kOuterTokens / 32; ++b) {
-      if (b * 32 < left_now) {
+    for (int b = 0; b < NB; ++b) {
+      if (k0 + b * 32 < left_now) {
         if (!whole)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            settle(q[b][e], static_cast<int64_t>(t_now + min(b * 32 + g * 8 + e, left_now - 1)) * ldx + j, xall);
-        if (b * 32 + 32 > left_now)                          // no tokens of other segments
+            settle(q[b][e], static_cast<int64_t>(t_now + min(k0 + b * 32 + g * 8 + e, left_now - 1)) * ldx + j, xall);
+        if (k0 + b * 32 + 32 > left_now)                     // no tokens of other segments
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (b * 32 + g * 8 + e >= left_now) q[b][e] = RawN<T, PC>{};
+            if (k0 + b * 32 + g * 8 + e >= left_now) q[b][e] = RawN<T, PC>{};
         Frag<T, T> fx[PC];
 #pragma unroll
         for (int a = 0; a < PC; ++a) fx[a] = column_of<T, T>(q[b], a);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const auto fh = SH::get(lds, r * 16 + n, b * 4 + g);
+          const auto fh = SH::get(lds, r * 16 + n, k0 / 8 + b * 4 + g);
 #pragma unroll
           for (int a = 0; a < PC; ++a) mma(acc[r][a], fh, fx[a]);
         }
       }
-      if (more && b * 32 < left) fetch(b);                   // the next stage's into the registers just read
+      if (more && k0 + b * 32 < left) fetch(b);                   // the next stage's into the registers just read
     }
+  }
+  if constexpr (SPLIT) {                                     // (0 + 2) + (1 + 3)
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half)
+#pragma unroll
+        for (int p = 0; p < RT * PC; ++p) sums[((wave - half) * RT * PC + p) * 64 + lane] = acc[p / PC][p % PC];
+      __syncthreads();
+      if (wave < half)
+#pragma unroll
+        for (int p = 0; p < RT * PC; ++p) acc[p / PC][p % PC] += sums[(wave * RT * PC + p) * 64 + lane];
+    }
+    if (wave != 0) return;
   }
   const bool any = it.any;
   const bool last = gridDim.z == 1;
@@ -924,8 +942,8 @@ static int check_common(const Segs& sg, const Shape& sh, const void* x, int64_t 
   SRA_REQUIRE(wdtype == SRA_F32 || wdtype == dtype, SRA_ERR_ARG,
               "wdtype must be SRA_F32 or the activations' dtype, got %d", wdtype);
   SRA_REQUIRE((x != nullptr || sg.tokens == 0) && A != nullptr && B != nullptr, SRA_ERR_ARG, "x, A and B must be non-null");
-  SRA_REQUIRE(sh.k >= 1 && sh.m >= 1 && sh.k < (int64_t{1} << 31) && sh.m < (int64_t{1} << 31), SRA_ERR_SHAPE,
-              "k and m must be in [1, 2^31), got %lld, %lld", static_cast<long long>(sh.k),
+  SRA_REQUIRE(sh.k >= 1 && sh.m >= 1 && sh.k < (int64_t{1} << 28) && sh.m < (int64_t{1} << 28), SRA_ERR_SHAPE,
+              "k and m must be in [1, 2^28), got %lld, %lld", static_cast<long long>(sh.k),
               static_cast<long long>(sh.m));
   SRA_REQUIRE(sh.rank >= 1, SRA_ERR_ARG, "rank must be >= 1, got %d", sh.rank);
   SRA_REQUIRE(sh.rank <= SRA_ADAPTER_MAX_RANK, SRA_ERR_UNSUPPORTED, "rank %d is above %d", sh.rank,
@@ -955,11 +973,15 @@ static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
   return p;
 }
 
+// Whether outer's waves share their columns: where whole workgroups' columns give
+// fewer than one workgroup a compute unit.
+static bool outer_split(int nslots, int64_t width) { return cdiv(width, 64 * kOuterCols) * nslots < 256; }
+
 // Parts of a client's tokens that outer sums apart: four workgroups a compute
 // unit, each with at least 2 stages of tokens on average (clients with more hold
 // the launch up less, the join costs a pass over the parts).
 static int outer_parts(int64_t tokens, int nslots, int64_t width) {
-  const int64_t blocks = cdiv(width, 64 * kOuterCols) * nslots;
+  const int64_t blocks = cdiv(width, (outer_split(nslots, width) ? 16 : 64) * kOuterCols) * nslots;
   const int64_t stages = cdiv(tokens, kOuterTokens * static_cast<int64_t>(nslots));
   int p = 1;
   while (p < kMaxParts && blocks * p < 1024 && stages >= 2 * p) p *= 2;
@@ -999,6 +1021,7 @@ template <typename T, typename W, bool AT>
 static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw, const Segs& sg, int64_t width,
                          int parts, int rank, float* H, hipStream_t st) {
   if (width < 8) {
+    if (int rc = check_launch(sg.tokens, 256)) return rc;
     hipLaunchKernelGGL((tiny_shrink_kernel<T, W>), dim3(static_cast<unsigned>(sg.tokens)), dim3(256), 0, st,
                        static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, AT ? 1 : width,
                        AT ? static_cast<int64_t>(rank) : 1, sg, static_cast<int>(width), rank, H);
@@ -1007,6 +1030,7 @@ static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw,
   return with_tile(sg, rank, [&](auto nt, auto rt) {
     constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, KB = kShrinkCols<T, RT, NT>;
     const int part = static_cast<int>(cdiv(cdiv(width, parts), KB) * KB);
+    if (int rc = check_launch(static_cast<int64_t>(tile_count<16 * NT>(sg)) * parts, kThreads)) return rc;
     hipLaunchKernelGGL((shrink_kernel<T, W, RT, NT, AT>), dim3(tile_count<16 * NT>(sg) * parts), dim3(kThreads), 0, st,
                        static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, sg, static_cast<int>(width),
                        parts, part, rank, H);
@@ -1019,6 +1043,7 @@ static int launch_expand(const void* base, int64_t ldb, const float* H, int part
                          const Segs& sg, int64_t width, int rank, float scale, void* out, int64_t ldo, float* Hsum,
                          hipStream_t st) {
   if (width < 8) {
+    if (int rc = check_launch(sg.tokens, 256)) return rc;
     if (parts > 1 || Hsum != nullptr) {
       float* sum = Hsum != nullptr ? Hsum : const_cast<float*>(H);
       const int64_t all = sg.tokens * rank;
@@ -1040,6 +1065,7 @@ static int launch_expand(const void* base, int64_t ldb, const float* H, int part
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, tiles), cdiv(width, COLS)));
     const int span = static_cast<int>(cdiv(cdiv(width, want), COLS) * COLS);
     const int blocks = static_cast<int>(cdiv(width, span));
+    if (int rc = check_launch(static_cast<int64_t>(tiles) * blocks, kThreads)) return rc;
     auto go = [&](auto rp) {
       constexpr int RP = decltype(rp)::value;
       hipLaunchKernelGGL((expand_kernel<T, W, RP, NT, AT>), dim3(static_cast<unsigned>(tiles) * blocks),
@@ -1066,11 +1092,16 @@ static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& 
   const int64_t per = rank * width, stride = per * sg.nslots;
   const int rc = with_tile(sg, rank, [&](auto, auto rt) {
     constexpr int RT = decltype(rt)::value;
-    const dim3 grid(static_cast<unsigned>(cdiv(width, 64 * kOuterCols)), static_cast<unsigned>(sg.nslots), parts);
-    hipLaunchKernelGGL((outer_kernel<T, RT, AT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx, H, sg,
-                       static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg, stride,
-                       accumulate);
-    return launch_status("outer_kernel");
+    auto go = [&](auto split) {
+      constexpr bool SPLIT = decltype(split)::value;
+      const dim3 grid(static_cast<unsigned>(cdiv(width, (SPLIT ? 16 : 64) * kOuterCols)),
+                      static_cast<unsigned>(sg.nslots), parts);
+      hipLaunchKernelGGL((outer_kernel<T, RT, AT, SPLIT>), grid, dim3(kThreads), 0, st, static_cast<const T*>(x), ldx,
+                         H, sg, static_cast<int>(width), rank, scale, parts > 1 ? parts_ws : G, parts > 1 ? per : ldg,
+                         stride, accumulate);
+      return launch_status("outer_kernel");
+    };
+    return outer_split(sg.nslots, width) ? go(std::true_type{}) : go(std::false_type{});
   });
   if (rc || parts == 1) return rc;
   const dim3 jg(static_cast<unsigned>(cdiv(per, 1024)), static_cast<unsigned>(sg.nslots));
@@ -1159,8 +1190,8 @@ extern "C" int sra_adapter_workspace_bytes(int64_t tokens, int32_t nseg, int32_t
   SRA_REQUIRE(bytes != nullptr, SRA_ERR_ARG, "null bytes pointer");
   if (int rc = check_tokens(tokens, nslots)) return rc;
   SRA_REQUIRE(nseg >= 0, SRA_ERR_ARG, "nseg must be >= 0, got %d", nseg);
-  SRA_REQUIRE(k >= 1 && m >= 1 && k < (int64_t{1} << 31) && m < (int64_t{1} << 31), SRA_ERR_SHAPE,
-              "k and m must be in [1, 2^31), got %lld, %lld", static_cast<long long>(k), static_cast<long long>(m));
+  SRA_REQUIRE(k >= 1 && m >= 1 && k < (int64_t{1} << 28) && m < (int64_t{1} << 28), SRA_ERR_SHAPE,
+              "k and m must be in [1, 2^28), got %lld, %lld", static_cast<long long>(k), static_cast<long long>(m));
   SRA_REQUIRE(rank >= 1, SRA_ERR_ARG, "rank must be >= 1, got %d", rank);
   SRA_REQUIRE(rank <= SRA_ADAPTER_MAX_RANK, SRA_ERR_UNSUPPORTED, "rank %d is above %d", rank,
               SRA_ADAPTER_MAX_RANK);
@@ -1217,6 +1248,7 @@ extern "C" int sra_adapter_grad(const void* dout, int64_t lddo, const void* x, i
   if (int rc = sra_adapter_workspace_bytes(tokens, nseg, nslots, k, m, rank, &need)) return rc;
   SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "adapter workspace: need %zu bytes, got %zu", need,
               ws_bytes);
+  SRA_REQUIRE(dx == nullptr || (dx != dout && dx != x), SRA_ERR_ARG, "dx must not be dout or x: they are read after it");
   const GradOut g{hidden, dxbase, lddxb, dx, lddx, dA, ldda, dB, lddb, accumulate};
   const Weights wt{A, lda, B, ldb};
   return with_types(dtype, wdtype, [&](auto t, auto w) {

@@ -190,26 +190,31 @@ __global__ void __launch_bounds__(kSortThreads) sort_tiles_kernel(Tokens k, int6
   for (int i = threadIdx.x; i < n; i += kSortThreads) keys[t0 + i] = buf[cur][i];
 }
 
-// Sorted tiles into one sorted list: an element's place is its place in its own
-// tile plus the count of smaller elements of every other tile, 4 searches in step.
-__global__ void __launch_bounds__(256) merge_tiles_kernel(const uint64_t* __restrict__ keys, int tokens, int tiles,
-                                                          uint64_t* __restrict__ sorted) {
-  const int i = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+// Sorted runs, kGroup neighbours into one: an element's place is its place in its
+// own run plus the count of smaller elements of the other runs, 4 searches in
+// step.  More runs than a group take more passes: all against all would cost
+// their square.
+// ---------------------------------------------------------------------------
+constexpr int kGroup = 16;
+
+__global__ void __launch_bounds__(256) merge_runs_kernel(const uint64_t* __restrict__ keys, int64_t tokens,
+                                                         int64_t run, uint64_t* __restrict__ sorted) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= tokens) return;
   const uint64_t key = keys[i];
-  const int mine = i / kTile;
-  int place = i - mine * kTile;
-  for (int q0 = 0; q0 < tiles; q0 += 4) {
-    int64_t at[4], from[4];
-    int n[4];
+  const int64_t mine = i / run, first = mine / kGroup * kGroup;
+  const int64_t end = min(first + kGroup, (tokens + run - 1) / run);
+  int64_t place = first * run + i - mine * run;
+  for (int64_t q0 = first; q0 < end; q0 += 4) {
+    int64_t at[4], from[4], n[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      from[q] = at[q] = static_cast<int64_t>(min(q0 + q, tiles - 1)) * kTile;
-      const bool search = q0 + q < tiles && q0 + q != mine;
-      n[q] = search ? static_cast<int>(min(static_cast<int64_t>(kTile), tokens - at[q])) : 0;
+      from[q] = at[q] = min(q0 + q, end - 1) * run;
+      const bool search = q0 + q < end && q0 + q != mine;
+      n[q] = search ? min(run, tokens - at[q]) : 0;
     }
     // keys at and beyond n count as larger
-    for (int step = kTile / 2; step > 0; step >>= 1)
+    for (int64_t step = run / 2; step > 0; step >>= 1)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int64_t probe = at[q] + step - 1;
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(256) merge_tiles_kernel(const uint64_t* __rest
     for (int q = 0; q < 4; ++q) {
       const bool in = at[q] - from[q] < n[q];
       if (in && keys[in ? at[q] : from[q]] < key) ++at[q];
-      place += static_cast<int>(at[q] - from[q]);
+      place += at[q] - from[q];
     }
   }
   sorted[place] = key;
@@ -452,7 +457,9 @@ extern "C" int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const i
       using T = decltype(t);
       // 16 lanes a token unless that leaves the card less than 4 waves a compute unit
       const bool few = tokens * 16 < 64 * 1024;
-      const dim3 grid(static_cast<unsigned>(cdiv(tokens * (few ? 64 : 16), 256)));
+      const int64_t blocks = cdiv(tokens * (few ? 64 : 16), 256);
+      if (int rc = check_launch(blocks, 256)) return rc;
+      const dim3 grid(static_cast<unsigned>(blocks));
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const W*>(table),
                            ldt, k, scale, static_cast<T*>(out), ldo);
@@ -496,25 +503,32 @@ extern "C" int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, con
   Clear clear{grad, ldg, vocab * dim, 0};
   if (!accumulate) {
     // one store a thread (983 MB: 156 us, against 172 us with 15 stores a thread),
-    // more only where that would be too many workgroups for a launch
+    // more only where that would be too many workgroups for a launch (above 32 GiB)
     const int64_t most = cdiv(clear.per, kSortThreads * 4);
-    clear.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (int64_t{1} << 30) / nslots)));
+    clear.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (int64_t{1} << 21) / nslots)));
   }
   if (tiles == 0 && accumulate) return SRA_OK;
   const int64_t blocks = tiles + static_cast<int64_t>(clear.blocks) * nslots;
-  SRA_REQUIRE(blocks < (int64_t{1} << 31), SRA_ERR_UNSUPPORTED, "%d slots are too many", nslots);
-  hipLaunchKernelGGL(sort_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), 0, st, k, padding,
-                     tiles, tiles > 1 ? keys : sorted, clear);
-  if (int rc = launch_status("sort_tiles_kernel")) return rc;
-  if (tokens == 0) return SRA_OK;
-  if (tiles > 1) {
-    hipLaunchKernelGGL(merge_tiles_kernel, dim3(static_cast<unsigned>(cdiv(tokens, 256))), dim3(256), 0, st, keys,
-                       static_cast<int>(tokens), tiles, sorted);
-    if (int rc = launch_status("merge_tiles_kernel")) return rc;
-  }
+  if (int rc = check_launch(blocks, kSortThreads)) return rc;
   const int chunks = static_cast<int>(cdiv(dim, kCols));
   const int window = window_of(tokens, dim);
   const int64_t units = cdiv(tokens, window) * chunks;
+  if (int rc = check_launch(cdiv(units, 4), 256)) return rc;
+  // the passes end in `sorted`
+  int passes = 0;
+  for (int64_t run = kTile; run < tokens; run *= kGroup) ++passes;
+  uint64_t* src = passes % 2 ? keys : sorted;
+  hipLaunchKernelGGL(sort_tiles_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), 0, st, k, padding,
+                     tiles, src, clear);
+  if (int rc = launch_status("sort_tiles_kernel")) return rc;
+  if (tokens == 0) return SRA_OK;
+  for (int64_t run = kTile; run < tokens; run *= kGroup) {
+    uint64_t* dst = src == keys ? sorted : keys;
+    hipLaunchKernelGGL(merge_runs_kernel, dim3(static_cast<unsigned>(cdiv(tokens, 256))), dim3(256), 0, st, src,
+                       tokens, run, dst);
+    if (int rc = launch_status("merge_runs_kernel")) return rc;
+    src = dst;
+  }
   const dim3 grid(static_cast<unsigned>(cdiv(units, 4)));
   const Grad o{grad, ldg, scale, accumulate};
   const int rc = with_type(dtype, [&](auto t) {

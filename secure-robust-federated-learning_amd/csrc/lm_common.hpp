@@ -81,6 +81,14 @@ inline int check_segments(const int64_t* offsets, const int32_t* slots, int32_t 
   return SRA_OK;
 }
 
+// A launch holds fewer than 2^32 threads a dimension.
+inline int check_launch(int64_t blocks, int threads) {
+  SRA_REQUIRE(blocks * threads < (int64_t{1} << 32), SRA_ERR_UNSUPPORTED,
+              "%lld workgroups of %d threads are too many for one launch: split the rows",
+              static_cast<long long>(blocks), threads);
+  return SRA_OK;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 unsigned int adapter_row_faults(bool reset);

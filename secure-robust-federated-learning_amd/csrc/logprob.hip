@@ -514,6 +514,7 @@ template <typename T, int WAVES, int KEEP>
 static int launch_rows(const void* logits, const Args& a, void* grad, hipStream_t st) {
   constexpr int kRows = WAVES < 4 ? 4 / WAVES : 1;
   const dim3 grid(static_cast<unsigned>(cdiv(a.rows, kRows))), block(WAVES < 4 ? 256 : WAVES * 64);
+  if (int rc = check_launch(grid.x, static_cast<int>(block.x))) return rc;
   const T* l = static_cast<const T*>(logits);
   T* g = static_cast<T*>(grad);
   if (g != nullptr) {
@@ -593,6 +594,7 @@ extern "C" int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t 
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(cdiv(vocab, kGradSpan)));
+    if (int rc = check_launch(rows, 256)) return rc;
     hipLaunchKernelGGL((logprob_grad_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
                        static_cast<const T*>(logits), a, lse, entropy, static_cast<T*>(grad));
     return launch_status("logprob_grad_kernel");

@@ -202,9 +202,10 @@ def adapter_grad(grad_out, x, A, B, offsets, slots, scale=1.0, hidden=None, base
     dx = base_grad + scale * A' B' grad_out (x's type; base_grad, the shared
     projection's part, None for zeros); dA (n, r, K) and dB (n, M, r) are float32.
     Each of grad_x, grad_A, grad_B is True (a new tensor), False (None returned) or
-    the tensor to write; grad_x may be base_grad.  Every slot of dA and dB is
-    written, zeros where it has no token; accumulate=True adds to the tensors given
-    instead.  ``hidden`` is adapter_apply's, or None to compute it again."""
+    the tensor to write; grad_x may be base_grad, but not grad_out or x.  Every slot
+    of dA and dB is written, zeros where it has no token; accumulate=True adds to the
+    tensors given instead.  ``hidden`` is adapter_apply's, or None to compute it
+    again."""
     head, keep, T, K, M, n, r, dtype, wdtype = _adapter_args(x, A, B, offsets, slots)
     dev = x.device
     dy, lddy = _rows("grad_out", grad_out, (T, M), x.dtype, dev)

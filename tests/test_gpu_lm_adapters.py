@@ -282,3 +282,82 @@ def test_autograd_matches_the_formula_and_differences():
         lo[i], hi[i] = args[i] - 1e-4 * v, args[i] + 1e-4 * v
         diff = (loss(*hi) - loss(*lo)) / 2e-4              # the loss is quadratic at most in one argument
         assert abs((ref.d(leaf.grad) * v).sum().item() - diff) <= 1e-4 * max(1.0, abs(diff))
+
+
+@pytest.mark.parametrize("T,count,step,dtype,wdtype", [
+    (300, 255, 1, "bf16", "fp32"), (300, 256, 1, "fp32", "fp32"), (9000, 5000, 1, "bf16", "fp32"),
+    (9000, 257, 35, "bf16", "bf16"), (9000, 258, 34, "fp32", "fp32"),
+])
+def test_more_segments_than_one_round_of_loads(T, count, step, dtype, wdtype):
+    """Segments of `step` tokens with empty ones and rows of no segment between them."""
+    g = torch.Generator().manual_seed(count)
+    sizes = step * torch.ones(count, dtype=torch.int64)
+    sizes[torch.randperm(count, generator=g)[:count // 5]] = 0
+    offsets = [2] + (2 + sizes.cumsum(0)).clamp(max=T).tolist()
+    slots = torch.randint(-1, 5, (count,), generator=g).tolist()
+    check(T, 24, 16, 3, 5, offsets, slots, dtype, wdtype)
+
+
+@pytest.mark.parametrize("T,K,M,r,n,dtype", [
+    (2000, 75, 64, 16, 1, "bf16"),        # few columns in all: waves share columns, parts of the tokens
+    (1500, 33, 300, 40, 2, "fp32"),
+    (700, 515, 8, 4, 100, "bf16"),        # a wave its own columns, the last ones of a row not whole
+    (33000, 513, 24, 8, 100, "fp16"),     # the same, parts of the tokens
+])
+def test_gradient_sums_split_over_workgroups(T, K, M, r, n, dtype):
+    slots = [n - 1, 0, 1 % n] + list(range(2, n - 1))          # the last ones are empty
+    offsets = [0, T // 3, T // 3 + 1, T - 5] + [T - 5] * (len(slots) - 3)
+    x, base, A, B, dy, dxb = make(T, K, M, r, n, DT[dtype], torch.float32)
+    o, s = seg(offsets, slots)
+    want = ref.adapter(base, x, A, B, offsets, slots, 0.5, DT[dtype], dy, dxb)
+    _, gA, gB = lm.adapter_grad(dy, x, A, B, o, s, 0.5)
+    ref.within("dA", gA, *want["dA"])
+    ref.within("dB", gB, *want["dB"])
+    gA, gB = torch.full_like(gA, 5.0), torch.full_like(gB, 5.0)
+    lm.adapter_grad(dy, x, A, B, o, s, 0.5, grad_A=gA, grad_B=gB, accumulate=True)
+    for name, got, (val, err) in (("dA", gA, want["dA"]), ("dB", gB, want["dB"])):
+        ref.within(name + " added", got, val + 5.0, err + 2 * ref.U * (val.abs() + 5.0))
+    for c in range(n):
+        if all(q != c or offsets[i] == offsets[i + 1] for i, q in enumerate(slots)):
+            assert (gA[c] == 5.0).all() and (gB[c] == 5.0).all()
+
+
+def test_rows_far_apart():
+    """Row strides that put offsets beyond 2^31 elements."""
+    T, K, M = 20, 40, 24
+    ld = (1 << 31) // 16
+    x, base, A, B, dy, dxb = make(T, K, M, 4, 2, torch.bfloat16, torch.float32)
+    o, s = seg([0, 7, 20], [1, 0])
+    far = torch.empty(T * ld, dtype=torch.bfloat16, device="cuda").view(T, ld)
+    fx, fb, fy, fo, fd = (far[:, i * 64:][:, :w] for i, w in enumerate((K, M, M, M, K)))
+    fx.copy_(x), fb.copy_(base), fy.copy_(dy)
+    y = lm.adapter_apply(base, x, A, B, o, s)
+    lm.adapter_apply(fb, fx, A, B, o, s, out=fo)
+    assert torch.equal(fo, y)
+    near = lm.adapter_grad(dy, x, A, B, o, s)
+    dx, gA, gB = lm.adapter_grad(fy, fx, A, B, o, s, grad_x=fd)
+    assert torch.equal(fd, near[0]) and torch.equal(gA, near[1]) and torch.equal(gB, near[2])
+
+
+def test_two_graphs_and_eager_calls_in_turn():
+    """Each graph has workspaces of its own."""
+    cases = []
+    for i, (T, n) in enumerate([(300, 3), (2100, 1)]):
+        x, base, A, B, dy, dxb = make(T, 640, 520, 8, n, torch.bfloat16, torch.float32, seed=i)
+        o, s = seg([0, T // 2, T], [n - 1, 0])
+        lm.adapter_apply(base, x, A, B, o, s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, h = lm.adapter_apply(base, x, A, B, o, s, hidden=True)
+            got = (y,) + lm.adapter_grad(dy, x, A, B, o, s, hidden=h, base_grad=dxb)
+        cases.append((graph, got, (x, base, A, B, dy, dxb, o, s)))
+    for _ in range(3):
+        for graph, got, _ in cases:
+            for t in got:
+                t.fill_(float("nan"))
+            graph.replay()
+        for _, got, (x, base, A, B, dy, dxb, o, s) in cases:
+            y, h = lm.adapter_apply(base, x, A, B, o, s, hidden=True)
+            for a, b in zip(got, (y,) + lm.adapter_grad(dy, x, A, B, o, s, hidden=h, base_grad=dxb)):
+                assert torch.equal(a, b)

@@ -166,3 +166,37 @@ def test_autograd():
     (lm.embedding(table, ids, scale=2.0, dtype=torch.bfloat16) * dy).sum().backward()
     want, bound = ref.embed_grad(dy, ids, 1, 11, None, None, 2.0)
     ref.within("table.grad", table.grad, want[0], bound[0])
+
+
+@pytest.mark.parametrize("T", [20000, 65536, 65537, 150001])
+def test_gradient_of_more_tokens_than_one_merge_takes(T):
+    """Runs of 4096 sorted tokens meet 16 at a time."""
+    V, E = 700, 9
+    dy, ids = rand(T, E, dtype=torch.bfloat16), ids_of(T, V)
+    ids[::3] = torch.randint(0, V, ((T + 2) // 3,), generator=torch.Generator().manual_seed(3))
+    ids = ids.cuda()
+    offsets, slots = [1, T // 4, T // 2, T - 2], [1, 0, 1]
+    o, s = seg(offsets, slots)
+    grad = torch.full((2, V, E), 7.0, device="cuda")
+    lm.embed_grad(dy, ids, grad, o, s, scale=0.5, padding_idx=3)
+    want, bound = ref.embed_grad(dy, ids, 2, V, offsets, slots, 0.5, padding=3)
+    ref.within("grad", grad, want, bound)
+    # whole numbers add up without rounding: every token is in its row once
+    ones = torch.ones(T, E, dtype=torch.bfloat16, device="cuda")
+    lm.embed_grad(ones, ids, grad, o, s, padding_idx=3)
+    want, _ = ref.embed_grad(ones, ids, 2, V, offsets, slots, 1.0, padding=3)
+    assert torch.equal(grad.cpu().double(), want)
+
+
+def test_many_segments():
+    T, V, E, n = 3000, 40, 16, 6
+    g = torch.Generator().manual_seed(2)
+    offsets = torch.randint(0, T + 1, (901,), generator=g).sort().values.tolist()
+    slots = torch.randint(-1, n, (900,), generator=g).tolist()
+    o, s = seg(offsets, slots)
+    table, ids, dy = rand(n, V, E), ids_of(T, V).cuda(), rand(T, E, dtype=torch.float16)
+    slot = ref.token_slots(offsets, slots, T).cuda()
+    want = torch.where((slot >= 0)[:, None], table[slot.clamp(min=0), ids] * 0.25, 0.0)
+    assert torch.equal(lm.embed(table, ids, o, s, scale=0.25), want)
+    grad = lm.embed_grad(dy, ids, torch.empty(n, V, E, device="cuda"), o, s)
+    ref.within("grad", grad, *ref.embed_grad(dy, ids, n, V, offsets, slots, 1.0))

@@ -138,3 +138,30 @@ def test_zero_rows_and_tokens_need_no_launch():
     _lib.call("sra_token_logprobs", None, 100, 1, None, 0, 100, -100, 0, None, None, None, None, None, None, None, None,
               0, None)
     _lib.call("sra_embed", P, 8, 0, None, None, None, 0, 0, 1, 4, 2, 1.0, None, 2, 0, None)
+
+
+def test_launches_too_large_are_refused_before_any_kernel():
+    """Counts that pass the checks of shapes but not what one launch holds."""
+    many, ws = 1 << 30, 1 << 60
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_adapter_apply", *adapter_args(tokens=many, ws_bytes=ws))
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_adapter_apply", *adapter_args(tokens=1 << 25, k=4, m=4, rank=1, ws_bytes=ws))
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_embed", P, 512, 0, P, None, None, 0, many, 1, 64, 8, 1.0, P, 8, 1, None)
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_embed_grad", P, 4096, 1, P, None, None, 0, many, 1, 64, 4096, 1.0, -1, P, 1 << 18, 0, P, ws, None)
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_token_logprobs", P, 100, 1, P, many, 100, -100, 0, P, None, P, None, None, None, None, None, 0,
+                  None)
+    with pytest.raises(NotImplementedError, match="too many"):
+        _lib.call("sra_token_logprobs_grad", P, 100, 1, P, many, 100, -100, P, None, P, None, P, 100, None)
+
+
+@pytest.mark.parametrize("alias", ["dout", "x"])
+def test_adapter_grad_refuses_dx_over_what_it_reads_later(alias):
+    p = {q: ctypes.c_void_p(4096 * (i + 1)) for i, q in enumerate(("dout", "x", "dx"))}
+    p["dx"] = p[alias]
+    with pytest.raises(ValueError, match="dx must not be"):
+        _lib.call("sra_adapter_grad", p["dout"], 64, p["x"], 64, P, 512, P, 512, P, P, 2, 8, 4, 64, 64, 8, 1.0, 1, 0,
+                  None, None, 0, p["dx"], 64, P, 512, P, 512, 0, P, BIG, None)

@@ -10,13 +10,15 @@
 // exchanged, so shrink and expand take a weight stored either way round.
 //
 // Arithmetic.  Sums are float32.  16-bit activations run on the bf16 units
-// (v_mfma_f32_16x16x32_bf16): bf16 values as they are, float32 and fp16 ones
-// (weights, h, z, fp16 activations) as two bf16 terms, the nearest and the rest,
-// with the product of the two rests left out: 2^-16 of a product, far inside
-// the rounding of 16-bit activations, for at most three matrix instructions
-// where memory leaves room for more.  A product with an infinity is then the sum
-// of two that may have opposite signs: it comes out infinite or NaN.  float32 activations run on the float32
-// units (v_mfma_f32_16x16x4_f32).
+// (v_mfma_f32_16x16x32_bf16): a bf16 value is one term, an fp16 one two (the
+// nearest bf16 and the rest), a float32 one (weights, h, z) three, which hold all
+// its 24 bits, where the result stays float32 (h, z, the gradients of A and B),
+// and two where it is rounded to 16 bits anyway (out, dx).  Products of terms
+// below 2^-16 (or 2^-8) of the whole are left out.  Memory bounds all three
+// products, so the matrix instructions, up to five for one, have room.  A product
+// with an infinity is then the sum of several that may have opposite signs: it
+// comes out infinite or NaN.  float32 activations run on the float32 units
+// (v_mfma_f32_16x16x4_f32).
 //
 // Layout.  A lane (n = lane % 16, g = lane / 16) of a 16x16 product holds row or
 // column n of its operands with the inner indices g * 8 .. g * 8 + 7 and, of the
@@ -185,25 +187,30 @@ struct Floats {
 };
 
 // the operand that T's matrix units take for stored values S
-template <typename T, typename S>
+template <typename T, typename S, bool FULL = false>
 using Frag = std::conditional_t<std::is_same_v<T, float>, Floats,
-                                Terms<std::is_same_v<S, __bf16> ? 1 : 2>>;
+                                Terms<std::is_same_v<S, __bf16> ? 1 : std::is_same_v<S, float> && FULL ? 3 : 2>>;
 
-// values e and e + 1, e even: the nearest bf16 and the rest
-__device__ __forceinline__ void put2(Terms<2>& f, int e, f32x2 x) {
-  const unsigned hi = pack2<__bf16>(x[0], x[1]);
-  const f32x2 h = unpack2<__bf16>(hi);
-  f.t[0][e / 2] = hi;
-  f.t[1][e / 2] = pack2<__bf16>(x[0] - h[0], x[1] - h[1]);
+// values e and e + 1, e even: the nearest bf16, that of the rest, that of its rest
+template <int N>
+__device__ __forceinline__ void put2(Terms<N>& f, int e, f32x2 x) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    f.t[i][e / 2] = pack2<__bf16>(x[0], x[1]);
+    if (i + 1 < N) {
+      const f32x2 h = unpack2<__bf16>(f.t[i][e / 2]);
+      x = f32x2{x[0] - h[0], x[1] - h[1]};
+    }
+  }
 }
 __device__ __forceinline__ void put2(Floats& f, int e, f32x2 x) {
   f.v[e] = x[0];
   f.v[e + 1] = x[1];
 }
 
-template <typename T, typename S>
-__device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
-  Frag<T, S> f;
+template <typename F, typename S>
+__device__ __forceinline__ F frag_of(const Raw8<S>& r) {
+  F f;
   if constexpr (std::is_same_v<S, __bf16>) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) f.t[0][b] = r.w[b];
@@ -215,9 +222,9 @@ __device__ __forceinline__ Frag<T, S> frag_of(const Raw8<S>& r) {
 }
 
 // column a of 8 rows
-template <typename T, typename S, int N>
-__device__ __forceinline__ Frag<T, S> column_of(const RawN<S, N> (&r)[8], int a) {
-  Frag<T, S> f;
+template <typename F, typename S, int N>
+__device__ __forceinline__ F column_of(const RawN<S, N> (&r)[8], int a) {
+  F f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     if constexpr (std::is_same_v<S, __bf16>)
@@ -263,15 +270,17 @@ __device__ __forceinline__ void get_frag(Floats& f, const u32x4* lds, int plane,
 template <typename F>
 constexpr int kPlanes = sizeof(F) / 16;
 
-template <int N, int M>
+// the products of the terms that add up to at least 2^-8 (FULL: 2^-16) of the whole
+template <bool FULL, int N, int M>
 __device__ __forceinline__ void mma(f32x4& acc, const Terms<N>& a, const Terms<M>& b) {
 #pragma unroll
   for (int i = N - 1; i >= 0; --i)
 #pragma unroll
     for (int j = M - 1; j >= 0; --j)
-      if (i + j < 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.term(i), b.term(j), acc, 0, 0, 0);
+      if (i + j < (FULL ? 3 : 2)) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.term(i), b.term(j), acc, 0, 0, 0);
 }
 
+template <bool FULL>
 __device__ __forceinline__ void mma(f32x4& acc, const Floats& a, const Floats& b) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
@@ -379,9 +388,9 @@ static int tile_count(const Segs& sg) {
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-template <typename T, typename S, int ROWS, int PIECES, bool TR, int PERM>
+template <typename T, typename S, int ROWS, int PIECES, bool TR, int PERM, bool FULL>
 struct Stage {
-  using F = Frag<T, S>;
+  using F = Frag<T, S, FULL>;
   static constexpr int kStep = PERM == 8 ? ROWS / 8 + 1 : PERM == 4 ? ROWS / 4 + 2 : 0;
   static constexpr int kPiece = PERM == 1 ? ROWS + 1 : PERM * kStep + (TR ? 4 : 1);
   static constexpr int kPlane = PIECES * kPiece;
@@ -452,13 +461,13 @@ struct Stage {
             for (int e = 0; e < 8; ++e) cut(r[q][e], c * 8 + e < inner ? 4 : 0);
           if (in)
 #pragma unroll
-            for (int a = 0; a < 4; ++a) put_frag(lds, kPlane, place(row + a, c), column_of<T, S>(r[q], a));
+            for (int a = 0; a < 4; ++a) put_frag(lds, kPlane, place(row + a, c), column_of<F>(r[q], a));
         }
       } else {
         const int k = u % PIECES * 8;
         if (near) settle(r[q][0], line_at(u), total);
         if (partial) cut(r[q][0], inner - k);
-        if (in) put_frag(lds, kPlane, place(u / PIECES, u % PIECES), frag_of<T, S>(r[q][0]));
+        if (in) put_frag(lds, kPlane, place(u / PIECES, u % PIECES), frag_of<F>(r[q][0]));
       }
     }
   }
@@ -478,16 +487,26 @@ struct Stage {
 // where the weight is the traffic): the waves share the stage's columns and their
 // sums meet in LDS in a fixed order.  W is [i][j] (AT false) or [j][i].
 // ---------------------------------------------------------------------------
-template <typename T, int RT, int NT>
-constexpr int kShrinkCols = NT == 1 ? 512 / RT : (RT == 4 || kPlanes<Frag<T, T>> == 2) ? 128 : 256;
+// Columns a stage: fewer where three terms of the weight take LDS and registers
+// from a second and third workgroup of the compute unit (bf16 activations, float32
+// weights: rank 64, 16384 x 8192, 64 columns 140 us, 128 180 us; rank 16, 6400 x
+// 2048, 128 columns 12.7 us, 256 15.7 us; one token of 100, 256 columns 10.5 us,
+// 512 12.9 us).
+template <typename T, typename W, int RT, int NT>
+constexpr int shrink_cols() {
+  const bool three = kPlanes<Frag<T, W, true>> == 3;
+  if (NT == 1) return three && RT < 4 ? 256 / RT : 512 / RT;
+  if (three) return RT == 4 ? 64 : 128;
+  return RT == 4 || kPlanes<Frag<T, T>> == 2 ? 128 : 256;
+}
 
 template <typename T, typename W, int RT, int NT, bool AT>
 __global__ void __launch_bounds__(kThreads)
     shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, Segs sg, int width,
                   int parts, int part, int rank, float* __restrict__ H) {
-  constexpr int KB = kShrinkCols<T, RT, NT>, PIECES = KB / 8;
-  using SX = Stage<T, T, 16 * NT, PIECES, false, 1>;
-  using SW = Stage<T, W, 16 * RT, PIECES, AT, AT ? 4 : 1>;
+  constexpr int KB = shrink_cols<T, W, RT, NT>(), PIECES = KB / 8;
+  using SX = Stage<T, T, 16 * NT, PIECES, false, 1, true>;
+  using SW = Stage<T, W, 16 * RT, PIECES, AT, AT ? 4 : 1, true>;
   __shared__ u32x4 lds[(SX::kBytes + SW::kBytes) / 16];
   u32x4* const ldw_ = lds + SX::kBytes / 16;
   const int tile = static_cast<int>(blockIdx.x) / parts, pt = static_cast<int>(blockIdx.x) % parts;
@@ -531,7 +550,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int r = 0; r < UR; ++r) {
         const auto fw = SW::get(ldw_, (rk + r) * 16 + n, b * 4 + g);
 #pragma unroll
-        for (int u = 0; u < UT; ++u) mma(acc[u][r], fw, fx[u]);
+        for (int u = 0; u < UT; ++u) mma<true>(acc[u][r], fw, fx[u]);
       }
     }
   }
@@ -579,7 +598,7 @@ __global__ void __launch_bounds__(kThreads)
                   int64_t ldw, Segs sg, int width, int blocks, int span, int rank, float scale, T* out, int64_t ldo,
                   float* __restrict__ Hsum) {
   constexpr int COLS = kExpandCols<NT>, PC = NT == 1 ? 4 : 8, RK = (RP + 3) / 4;
-  using SW = Stage<T, W, COLS, RP, !AT, PC>;                 // RP pieces of 8 ranks
+  using SW = Stage<T, W, COLS, RP, !AT, PC, false>;                 // RP pieces of 8 ranks
   __shared__ u32x4 lds[SW::kBytes / 16];
   const int tile = static_cast<int>(blockIdx.x) / blocks, block = static_cast<int>(blockIdx.x) % blocks;
   const Tile tl = find_tile<16 * NT>(sg, tile);
@@ -662,7 +681,7 @@ __global__ void __launch_bounds__(kThreads)
         // and so are their weights
         Frag<T, W> fw = SW::get(lds, row + a, RP < 4 ? min(g, RP - 1) : b * 4 + g);
         if (RP < 4 && g >= RP) fw = Frag<T, W>{};
-        mma(acc[a], fh[b], fw);
+        mma<false>(acc[a], fh[b], fw);
       }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -732,7 +751,7 @@ template <typename T, int RT, bool AT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads)
     outer_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ H, Segs sg, int width, int rank,
                  float scale, float* __restrict__ G, int64_t ldg, int64_t part_stride, int accumulate) {
-  using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true, 4>;
+  using SH = Stage<T, float, 16 * RT, kOuterTokens / 8, true, 4, true>;
   constexpr int PC = kOuterCols, NB = SPLIT ? 1 : kOuterTokens / 32, kSums = SPLIT ? 2 * RT * PC * 64 : 0;
   __shared__ u32x4 lds[SH::kBytes / 16 > kSums ? SH::kBytes / 16 : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -783,12 +802,12 @@ __global__ void __launch_bounds__(kThreads)
             if (k0 + b * 32 + g * 8 + e >= left_now) q[b][e] = RawN<T, PC>{};
         Frag<T, T> fx[PC];
 #pragma unroll
-        for (int a = 0; a < PC; ++a) fx[a] = column_of<T, T>(q[b], a);
+        for (int a = 0; a < PC; ++a) fx[a] = column_of<Frag<T, T>>(q[b], a);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const auto fh = SH::get(lds, r * 16 + n, k0 / 8 + b * 4 + g);
 #pragma unroll
-          for (int a = 0; a < PC; ++a) mma(acc[r][a], fh, fx[a]);
+          for (int a = 0; a < PC; ++a) mma<true>(acc[r][a], fh, fx[a]);
         }
       }
       if (more && k0 + b * 32 < left) fetch(b);                   // the next stage's into the registers just read
@@ -1028,7 +1047,7 @@ static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw,
     return launch_status("tiny_shrink_kernel");
   }
   return with_tile(sg, rank, [&](auto nt, auto rt) {
-    constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, KB = kShrinkCols<T, RT, NT>;
+    constexpr int NT = decltype(nt)::value, RT = decltype(rt)::value, KB = shrink_cols<T, W, RT, NT>();
     const int part = static_cast<int>(cdiv(cdiv(width, parts), KB) * KB);
     if (int rc = check_launch(static_cast<int64_t>(tile_count<16 * NT>(sg)) * parts, kThreads)) return rc;
     hipLaunchKernelGGL((shrink_kernel<T, W, RT, NT, AT>), dim3(tile_count<16 * NT>(sg) * parts), dim3(kThreads), 0, st,

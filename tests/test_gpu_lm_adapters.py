@@ -361,3 +361,26 @@ def test_two_graphs_and_eager_calls_in_turn():
             y, h = lm.adapter_apply(base, x, A, B, o, s, hidden=True)
             for a, b in zip(got, (y,) + lm.adapter_grad(dy, x, A, B, o, s, hidden=h, base_grad=dxb)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,M,r,offsets,slots", [
+    (70, 129, 257, 16, [0, 1, 34, 70], [2, 0, 1]), (200, 520, 260, 64, [0, 150, 200], [1, 0]),
+    (20, 300, 90, 24, list(range(21)), [i % 3 for i in range(20)]),
+])
+def test_float32_weights_and_gradients_keep_their_bits(T, K, M, r, offsets, slots, dtype, monkeypatch):
+    """Hidden values and gradients stay float32: three bf16 terms hold a float32's
+    24 bits, two an fp16's 11, and what is left out of their products is below
+    2^-8 * 2^-16 of one, twice: 2^-22 bounds it beside the float32 sums."""
+    monkeypatch.setattr(ref, "PROD", 2.0 ** -22)
+    x, base, A, B, dy, dxb = make(T, K, M, r, 3, DT[dtype], torch.float32)
+    o, s = seg(offsets, slots)
+    want = ref.adapter(base, x, A, B, offsets, slots, 0.7, DT[dtype], dy, dxb)
+    _, h = lm.adapter_apply(base, x, A, B, o, s, 0.7, hidden=True)
+    _, dA, dB = lm.adapter_grad(dy, x, A, B, o, s, 0.7, hidden=h)
+    ref.within("dA", dA, *want["dA"])
+    ref.within("dB", dB, *want["dB"])
+    for a, b, c in ref.segments(offsets, slots, T):
+        v, e = ref.product(ref.d(x[a:b]), torch.zeros(b - a, K).double(), ref.d(A[c]).T.contiguous(),
+                           torch.zeros(K, r).double())
+        ref.within("hidden", h[a:b], v, e)

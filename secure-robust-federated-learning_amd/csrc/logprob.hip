@@ -417,6 +417,8 @@ constexpr int kAhead = 4;                 // stretches a wave takes at a time
 
 // WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.  KEEP > 0: a wave
 // holds its up to KEEP stretches in registers from the one read to the gradient.
+// Bound by memory: 4096 rows of 50001 bf16 logits and their gradient 200 us (4.1
+// TB/s read and written; rows start at odd places), 249 us read twice.
 template <typename T, int WAVES, bool TOP, bool GRAD, int KEEP>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
     logprob_kernel(const T* logits, Args a, T* grad) {
@@ -635,8 +637,10 @@ static int launch_rows(const void* logits, const Args& a, void* grad, hipStream_
   return launch_status("logprob_kernel");
 }
 
-// Waves a row: one for rows of up to 2048 logits; 4 where the rows fill the card,
-// 16 where they do not.  With the gradient, 8 waves keep a row of up to 65536
+// Waves a row: one for rows of up to 2048 logits (4096 rows of 1024 5.2 us, 7.0 us
+// with 4 waves; 8 rows of 4096 6.3 us, 4.3 us with 16); 4 where the rows fill the
+// card, 16 where they do not (rows of 32768: 256 8.6 us with 4, 7.7 with 16; 512
+// 12.4, 13.9; 2048 34.7, 44.5).  With the gradient, 8 waves keep a row of up to 65536
 // 16-bit (32768 float32) logits in registers; longer ones are read twice.
 template <typename T>
 static int launch(const void* logits, const Args& a, void* grad, hipStream_t st) {
@@ -646,7 +650,7 @@ static int launch(const void* logits, const Args& a, void* grad, hipStream_t st)
     if (a.vocab <= 8 * kMost / 4 * kStretch) return launch_rows<T, 8, kMost / 4>(logits, a, grad, st);
     return launch_rows<T, 8, kMost>(logits, a, grad, st);
   }
-  return a.rows < 1024 ? launch_rows<T, 16, 0>(logits, a, grad, st) : launch_rows<T, 4, 0>(logits, a, grad, st);
+  return a.rows < 512 ? launch_rows<T, 16, 0>(logits, a, grad, st) : launch_rows<T, 4, 0>(logits, a, grad, st);
 }
 
 template <typename F>

@@ -240,6 +240,8 @@ def fl_round(network, store, choices, local_update, args, state=None, attack="no
     the parameters in place and returned as the flat (D,) device vector."""
     from . import attack as atk, dispatch
 
+    if bank is not None and bank.store is not store:
+        raise ValueError("the bank belongs to another store")
     store.snapshot()
     if bank is not None:
         bank.load(choices)

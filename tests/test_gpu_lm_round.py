@@ -211,3 +211,12 @@ def test_autograd_forms_refuse_capture():
             lm.embedding(table, ids)
     with torch.no_grad():
         assert lm.embedding(table, ids).shape == (5, E)
+
+
+def test_round_refuses_a_bank_of_another_store():
+    net = Net()
+    S, other = (store.ClientStore(net.parameters(), 4) for _ in range(2))
+    before = [p.clone() for p in net.params]
+    with pytest.raises(ValueError, match="another store"):
+        store.fl_round(net, S, [0, 1], lambda bank: bank.step(1.0), None, bank=store.ClientBank(other, 2))
+    assert all(torch.equal(p, q) for p, q in zip(net.params, before))

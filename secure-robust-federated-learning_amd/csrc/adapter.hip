@@ -993,11 +993,17 @@ constexpr int kMaxParts = 16;
 static int tile_groups(int64_t tokens, int nseg) { return tokens >= 32 * static_cast<int64_t>(nseg) ? 4 : 1; }
 
 // Parts of the width that shrink sums apart: two workgroups a compute unit where
-// the tiles alone give fewer, a part never below 512 columns.
-static int shrink_parts(int64_t tokens, int nseg, int64_t width) {
-  const int64_t tiles = tokens / (16 * tile_groups(tokens, nseg)) + std::min<int64_t>(nseg, tokens);
+// the tiles alone give fewer, a part never below 512 columns.  Where even one a
+// unit is out of reach, tiles of 64 tokens go down to 256 columns, or 128 at ranks
+// whose partial sums expand reads cheaply (a float32 step of 1501 tokens, 1001 ->
+// 777, rank 5: 70 us with 512, 60 with 256, 56 with 128; 2203 tokens, 960 -> 1216,
+// rank 19: 96, 85, 85; 2048 bf16 tokens, 1024 wide, rank 64: 23.5, 23.1, 25.9).
+static int shrink_parts(int64_t tokens, int nseg, int64_t width, int rank) {
+  const int groups = tile_groups(tokens, nseg);
+  const int64_t tiles = tokens / (16 * groups) + std::min<int64_t>(nseg, tokens);
+  const int64_t few = groups == 4 ? (rank <= 16 ? 256 : 512) : 1024;
   int p = 1;
-  while (p < kMaxParts && tiles * p < 512 && width >= 1024 * p) p *= 2;
+  while (p < kMaxParts && ((tiles * p < 256 && width >= few * p) || (tiles * p < 512 && width >= 1024 * p))) p *= 2;
   return p;
 }
 
@@ -1027,8 +1033,8 @@ static Workspace plan(int64_t tokens, int nseg, int nslots, int64_t k, int64_t m
   Workspace w{};
   w.h = 0;
   // expand may load up to 7 floats behind the parts of h or z
-  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, nseg, k) + 32;
-  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, nseg, m) + 1) + 32;
+  w.z = w.h + static_cast<size_t>(tokens) * row * shrink_parts(tokens, nseg, k, rank) + 32;
+  w.ga = w.z + static_cast<size_t>(tokens) * row * (shrink_parts(tokens, nseg, m, rank) + 1) + 32;
   w.gb = w.ga + (pa > 1 ? static_cast<size_t>(pa) * nslots * k * row : 0);
   w.bytes = w.gb + (pb > 1 ? static_cast<size_t>(pb) * nslots * m * row : 0) + 16;
   return w;
@@ -1154,7 +1160,7 @@ struct Weights {
 template <typename T, typename W>
 static int run_apply(const void* base, int64_t ldbase, const void* x, int64_t ldx, const Weights& w, const Segs& sg,
                      const Shape& sh, void* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
-  const int parts = shrink_parts(sg.tokens, sg.nseg, sh.k);
+  const int parts = shrink_parts(sg.tokens, sg.nseg, sh.k, sh.rank);
   float* H = reinterpret_cast<float*>(ws);
   if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, parts, sh.rank, H, st)) return rc;
   return launch_expand<T, W, true>(base, ldbase, H, parts, w.B, w.ldb, sg, sh.m, sh.rank, sh.scale, out, ldo,
@@ -1183,7 +1189,7 @@ static int run_grad(const void* dout, int64_t lddo, const void* x, int64_t ldx, 
   if (sg.tokens > 0) {
     if (g.dx != nullptr || g.dA != nullptr) {
       // the parts of z meet in the expand that needs them; without one there is one part
-      const int parts = g.dx != nullptr ? shrink_parts(sg.tokens, sg.nseg, sh.m) : 1;
+      const int parts = g.dx != nullptr ? shrink_parts(sg.tokens, sg.nseg, sh.m, sh.rank) : 1;
       float* Zp = Z;
       if (parts > 1) Z = Zp + static_cast<int64_t>(parts) * sg.tokens * sh.rank;
       if (int rc = launch_shrink<T, W, true>(dout, lddo, w.B, w.ldb, sg, sh.m, parts, sh.rank, Zp, st)) return rc;

@@ -384,3 +384,13 @@ def test_float32_weights_and_gradients_keep_their_bits(T, K, M, r, offsets, slot
         v, e = ref.product(ref.d(x[a:b]), torch.zeros(b - a, K).double(), ref.d(A[c]).T.contiguous(),
                            torch.zeros(K, r).double())
         ref.within("hidden", h[a:b], v, e)
+
+
+@pytest.mark.parametrize("T,K,M,r,dtype,wdtype", [
+    (700, 1001, 777, 5, "fp32", "fp32"), (300, 1024, 1500, 16, "bf16", "bf16"), (300, 1040, 2050, 16, "fp16", "fp32"),
+    (130, 4100, 520, 33, "bf16", "fp32"), (64, 9000, 300, 1, "bf16", "bf16"),
+])
+def test_few_tiles_share_the_width(T, K, M, r, dtype, wdtype):
+    """Hidden values as partial sums of the width, some parts of them empty."""
+    check(T, K, M, r, 2, [0, T // 2 + 3, T], [1, 0], dtype, wdtype)
+    check(T, K, M, r, 2, [0, T // 2 + 3, T], [1, 0], dtype, wdtype, base=False, hidden=False, pad_rows=1)

@@ -417,7 +417,7 @@ constexpr int kAhead = 4;                 // stretches a wave takes at a time
 
 // WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.  KEEP > 0: a wave
 // holds its up to KEEP stretches in registers from the one read to the gradient.
-// Bound by memory: 4096 rows of 50001 bf16 logits and their gradient 200 us (4.1
+// Bound by memory: 4096 rows of 50001 bf16 logits and their gradient 196 us (4.2
 // TB/s read and written; rows start at odd places), 249 us read twice.
 template <typename T, int WAVES, bool TOP, bool GRAD, int KEEP>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
@@ -640,15 +640,23 @@ static int launch_rows(const void* logits, const Args& a, void* grad, hipStream_
 // Waves a row: one for rows of up to 2048 logits (4096 rows of 1024 5.2 us, 7.0 us
 // with 4 waves; 8 rows of 4096 6.3 us, 4.3 us with 16); 4 where the rows fill the
 // card, 16 where they do not (rows of 32768: 256 8.6 us with 4, 7.7 with 16; 512
-// 12.4, 13.9; 2048 34.7, 44.5).  With the gradient, 8 waves keep a row of up to 65536
-// 16-bit (32768 float32) logits in registers; longer ones are read twice.
+// 12.4, 13.9; 2048 34.7, 44.5).  With the gradient, 8 waves keep a row of up to
+// 65536 16-bit (32768 float32) logits in registers, a quarter of them for rows a
+// quarter as long; longer rows are read twice.  4 waves with twice the registers
+// put three rows of 16-bit logits on a compute unit instead of two, where there are
+// that many (bf16, 32000 wide: 512 rows 25.6 us with 8, 27.7 with 4; 768 35.6, 33.4;
+// 4096 160, 141; 4096 of 5000 37.4, 29.9; float32 gains nothing).
 template <typename T>
 static int launch(const void* logits, const Args& a, void* grad, hipStream_t st) {
   constexpr int kMost = sizeof(T) == 4 ? 8 : 16;
   if (a.vocab <= 2048) return launch_rows<T, 1, 0>(logits, a, grad, st);
   if (grad != nullptr && a.vocab <= 8 * kMost * kStretch) {
-    if (a.vocab <= 8 * kMost / 4 * kStretch) return launch_rows<T, 8, kMost / 4>(logits, a, grad, st);
-    return launch_rows<T, 8, kMost>(logits, a, grad, st);
+    const bool quarter = a.vocab <= 8 * kMost / 4 * kStretch;
+    if constexpr (sizeof(T) == 2)
+      if (a.rows >= 768)
+        return quarter ? launch_rows<T, 4, kMost / 2>(logits, a, grad, st)
+                       : launch_rows<T, 4, 2 * kMost>(logits, a, grad, st);
+    return quarter ? launch_rows<T, 8, kMost / 4>(logits, a, grad, st) : launch_rows<T, 8, kMost>(logits, a, grad, st);
   }
   return a.rows < 512 ? launch_rows<T, 16, 0>(logits, a, grad, st) : launch_rows<T, 4, 0>(logits, a, grad, st);
 }

@@ -230,3 +230,16 @@ def test_evaluate_counts():
     want = ref.logprobs(x, t)
     assert int(kept) == 49 and int(right) == int(((best(x, 1)[:, 0] == t.cpu()) & (t.cpu() != -100)).sum())
     assert abs(float(loss) + float(want["logp"].sum())) <= 1e-3
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("R,V", [(767, 2049), (768, 2049), (769, 4099), (770, 16385)])
+def test_many_rows(R, V, dtype):
+    """Rows that fill the card, around the counts and lengths where a row's waves
+    change; the alternatives are those of the pass without a gradient."""
+    x, t = make(R, V, DT[dtype], seed=R)
+    check(x, t, 0, DT[dtype], seed=1)
+    a = lm.token_logprobs(x, t, top=3)
+    b, _ = lm.token_logprobs_and_grad(x, t, torch.ones(R, device="cuda"), top=3)
+    assert torch.equal(a.top_ids, b.top_ids)
+    assert torch.equal(x.gather(1, a.top_ids[:, :1]).squeeze(1), x.max(1).values)

@@ -209,8 +209,11 @@ def _own_adapters(st):
                                  hidden=True)
     dA = st["grads"][:, :r * K].view(n, r, K)
     dB = st["grads"][:, r * K:].view(n, M, r)
+    # float32 training adds to dx_base where it lies, as the plain form does (its conversion is no copy there)
+    in_place = st["dx_base"].dtype is torch.float32
     dx, _, _ = lm.adapter_grad(st["dy"], st["x"], st["A"], st["B"], st["offsets"], st["slots"], st["scale"],
-                               hidden=hidden, base_grad=st["dx_base"], grad_A=dA, grad_B=dB)
+                               hidden=hidden, base_grad=st["dx_base"], grad_x=st["dx_base"] if in_place else True,
+                               grad_A=dA, grad_B=dB)
     return y, dx, st["grads"]
 
 

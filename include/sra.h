@@ -550,8 +550,9 @@ int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t*
  * With grad (rows x vocab, dtype, row stride ldg; may equal logits) it also
  * writes the logits' gradient for given row gradients of logp and entropy:
  *   grad_i = grad_logp * (1[i = target] - p_i) - grad_entropy * p_i (log p_i + entropy)
- * (no logp part for an ignored target; grad_entropy may be NULL), which reads
- * the logits from memory once for both. */
+ * (no logp part for an ignored or bad target; grad_entropy may be NULL), which
+ * reads the logits from memory once for both.  A row whose parts are all absent
+ * or have the factor 0 gets zeros, whatever its logits are. */
 int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
                        int64_t vocab, int64_t ignore, int32_t top, float* logp, float* entropy, float* lse,
                        float* top_logp, int64_t* top_ids, const float* grad_logp, const float* grad_entropy,

@@ -386,15 +386,18 @@ struct RowGrad {
   bool same;                // logits and gradient are aligned alike
 
   __device__ __forceinline__ void operator()(float (&x)[kPer], int i, int valid) const {
-    float g[kPer];
+    float g[kPer] = {};
+    // nothing of a row that is left out, whatever it holds: 0 * p would be NaN with p
+    if (gl != 0.f || ge != 0.f) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const float l = x[e] - lse;
-      const float p = fast_exp(l);
-      float v = -gl * p;
-      if (ge != 0.f) v -= ge * p * (fmaxf(l, kFarBelow) + ent);
-      if (i + e == target) v += gl;
-      g[e] = v;
+      for (int e = 0; e < kPer; ++e) {
+        const float l = x[e] - lse;
+        const float p = fast_exp(l);
+        float v = -gl * p;
+        if (ge != 0.f) v -= ge * p * (fmaxf(l, kFarBelow) + ent);
+        if (i + e == target) v += gl;
+        g[e] = v;
+      }
     }
     if (valid == kPer && same) {
       store8(grow + i, g);

@@ -371,7 +371,9 @@ def token_logprobs_and_grad(logits, targets, grad_logp, grad_entropy=None, top=0
                             out=None):
     """``token_logprobs`` and the logits' gradient for given row gradients of logp
     and entropy (float32 (rows,)), in one pass over the logits: a mean loss over n
-    targets is grad_logp = -1 / n.  ``out`` may be the logits (in place)."""
+    targets is grad_logp = -1 / n.  Rows with an ignored or bad target, or with
+    grad_logp 0, get zeros (beside the entropy's part) whatever their logits are.
+    ``out`` may be the logits (in place)."""
     if grad_logp is None:
         raise ValueError("grad_logp is needed")
     return _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entropy, out)

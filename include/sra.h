@@ -544,7 +544,9 @@ int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t*
  * index first among equals, NaN above everything.  entropy (optional), lse,
  * logp: rows floats; top_logp / top_ids: rows x top, 0 <= top <=
  * min(vocab, SRA_TOKEN_MAX_TOP).  -inf logits have p = 0 and add nothing to
- * the entropy; a row of only -inf, or with +inf or NaN, gives NaN.  A target
+ * the entropy; a row of only -inf (whose lse is -inf), or with +inf or NaN, gives
+ * NaN.  logp is formed from differences of logits: what a row's logits have in
+ * common, however large, costs no digits.  A target
  * equal to ignore gives logp 0; one outside the vocabulary gives NaN and is
  * counted as a row fault.
  * With grad (rows x vocab, dtype, row stride ldg; may equal logits) it also
@@ -558,12 +560,24 @@ int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int
                        float* top_logp, int64_t* top_ids, const float* grad_logp, const float* grad_entropy,
                        void* grad, int64_t ldg, void* stream);
 
+/* The same, which also writes lse_rest (rows floats, may be NULL): what the
+ * rounding of lse left, so that lse + lse_rest is max + log sum exactly. */
+int sra_token_logprobs_split(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
+                             int64_t vocab, int64_t ignore, int32_t top, float* logp, float* entropy, float* lse,
+                             float* lse_rest, float* top_logp, int64_t* top_ids, const float* grad_logp,
+                             const float* grad_entropy, void* grad, int64_t ldg, void* stream);
+
 /* The same gradient from a forward pass's lse and entropy (entropy is needed
- * with grad_entropy only). */
+ * with grad_entropy only).  From lse alone every p of a row is off by up to
+ * 2^-24 |lse| of itself; _split takes lse_rest (may be NULL) too and is not. */
 int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
                             int64_t vocab, int64_t ignore, const float* lse, const float* entropy,
                             const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
                             void* stream);
+int sra_token_logprobs_grad_split(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
+                                  int64_t vocab, int64_t ignore, const float* lse, const float* lse_rest,
+                                  const float* entropy, const float* grad_logp, const float* grad_entropy, void* grad,
+                                  int64_t ldg, void* stream);
 
 #ifdef __cplusplus
 }

@@ -138,8 +138,12 @@ _SIGS = {
                        _ptr, _i64, _i32, _ptr, _sz, _ptr],
     "sra_token_logprobs": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
                            _ptr, _ptr, _i64, _ptr],
+    "sra_token_logprobs_split": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                 _ptr, _ptr, _ptr, _i64, _ptr],
     "sra_token_logprobs_grad": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64,
                                 _ptr],
+    "sra_token_logprobs_grad_split": [_ptr, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                      _i64, _ptr],
 }
 _RESTYPES = {"sra_last_error": ctypes.c_char_p}
 

@@ -6,8 +6,10 @@
 // joined over threads and waves by
 //   (m, s, u) + (m', s', u'):  with M = max(m, m'), d = m - M, f = e^d:
 //   s f + ...,  (u + s d) f + ...
-// so that  lse = m + log s,  logp = x_target - lse,  entropy = log s - u / s
-// without a difference of large numbers.
+// so that  lse = m + log s,  logp = (x_target - m) - log s,  entropy = log s - u / s
+// without a difference of large numbers.  lse is held as two floats, the rounded
+// sum and what its rounding left, so that x - lse keeps the digits of log s however
+// large the logits are (rows of float32's lowest value: log s next to 3.4e38).
 #include <type_traits>
 
 #include "lm_common.hpp"
@@ -42,6 +44,18 @@ __device__ __forceinline__ void join(Stats& a, Stats b) {
   rescale(b, M);
   a.s += b.s;
   a.u += b.u;
+}
+
+// m + log s in two floats, exactly: the larger addend comes back from the sum
+// without an error, and the other less that is what the rounding left.
+struct Lse {
+  float hi, lo;
+  __device__ __forceinline__ float below(float x) const { return (x - hi) - lo; }
+};
+
+__device__ __forceinline__ Lse lse_of(float m, float ls) {
+  const float hi = m + ls;
+  return {hi, fabsf(m) >= fabsf(ls) ? ls - (hi - m) : m - (hi - ls)};
 }
 
 template <int N>
@@ -370,6 +384,7 @@ struct Args {
   float* logp;
   float* entropy;
   float* lse;
+  float* lse_rest;
   float* top_logp;
   int64_t* top_ids;
   const float* grad_logp;
@@ -382,7 +397,8 @@ template <typename T>
 struct RowGrad {
   T* grow;
   int64_t target;
-  float lse, ent, gl, ge;
+  Lse lse;
+  float ent, gl, ge;
   bool same;                // logits and gradient are aligned alike
 
   __device__ __forceinline__ void operator()(float (&x)[kPer], int i, int valid) const {
@@ -391,7 +407,7 @@ struct RowGrad {
     if (gl != 0.f || ge != 0.f) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        const float l = x[e] - lse;
+        const float l = lse.below(x[e]);
         const float p = fast_exp(l);
         float v = -gl * p;
         if (ge != 0.f) v -= ge * p * (fmaxf(l, kFarBelow) + ent);
@@ -409,9 +425,13 @@ struct RowGrad {
   }
 };
 
+// A 16-bit gradient leaves the rest out where |lse| < 16: it moves p by less than
+// 2^-21 of itself (8 roundings of a float; the sums may have left as much), and the
+// gradient from lse alone then has the same bits.
 template <typename T>
-__device__ __forceinline__ RowGrad<T> row_grad(const T* row, T* grow, int64_t target, float lse, float ent, float gl,
+__device__ __forceinline__ RowGrad<T> row_grad(const T* row, T* grow, int64_t target, Lse lse, float ent, float gl,
                                                float ge) {
+  if (sizeof(T) == 2 && fabsf(lse.hi) < 16.f) lse.lo = 0.f;
   return {grow, target, lse, ent, gl, ge,
           ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0};
 }
@@ -521,7 +541,7 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
   }
   if (!live) return;
   const float ls = logf(st.s);
-  const float lse = st.m + ls;
+  const Lse lse = lse_of(st.m, ls);
   const float ent = ls - st.u / st.s;
   const int64_t target = a.targets[r];
   const bool ignored = target == a.ignore;
@@ -532,15 +552,16 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
       count_row_fault();
       lp = __builtin_nanf("");
     } else if (!ignored) {
-      lp = to_f32(row[target]) - lse;
+      lp = lse.below(to_f32(row[target]));
     }
     a.logp[r] = lp;
-    a.lse[r] = lse;
+    a.lse[r] = lse.hi;
+    if (a.lse_rest != nullptr) a.lse_rest[r] = lse.lo;
     if (a.entropy != nullptr) a.entropy[r] = ent;
   }
   if constexpr (TOP) {
     if (w == 0 && lane < a.top) {
-      a.top_logp[r * a.top + lane] = value_of(t.key) - lse;
+      a.top_logp[r * a.top + lane] = lse.below(value_of(t.key));
       a.top_ids[r * a.top + lane] = t.idx;
     }
   }
@@ -572,6 +593,7 @@ constexpr int kGradSpan = 8192;
 
 template <typename T>
 __global__ void __launch_bounds__(256) logprob_grad_kernel(const T* logits, Args a, const float* __restrict__ lse,
+                                                           const float* __restrict__ lse_rest,
                                                            const float* __restrict__ entropy, T* grad) {
   const int64_t r = blockIdx.x;
   const int from = blockIdx.y * kGradSpan;
@@ -587,7 +609,8 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(const T* logits, Args
   const float ge = a.grad_entropy != nullptr ? a.grad_entropy[r] : 0.f;
   const float ent = a.grad_entropy != nullptr ? entropy[r] : 0.f;
   const T* row = logits + r * a.ldl + from;
-  const auto put = row_grad(row, grad + r * a.ldg + from, target - from, lse[r], ent, gl, ge);
+  const Lse both{lse[r], lse_rest != nullptr ? lse_rest[r] : 0.f};
+  const auto put = row_grad(row, grad + r * a.ldg + from, target - from, both, ent, gl, ge);
   walk<1>(row, n, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 4,
           [&](float (&x)[1][kPer], int i, int, int valid) { put(x[0], i, valid); });
 }
@@ -675,11 +698,11 @@ static int with_type(int32_t dtype, F&& f) {
 
 using namespace sra;
 
-extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
-                                  int64_t rows, int64_t vocab, int64_t ignore, int32_t top, float* logp,
-                                  float* entropy, float* lse, float* top_logp, int64_t* top_ids,
-                                  const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
-                                  void* stream) {
+extern "C" int sra_token_logprobs_split(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                        int64_t rows, int64_t vocab, int64_t ignore, int32_t top, float* logp,
+                                        float* entropy, float* lse, float* lse_rest, float* top_logp,
+                                        int64_t* top_ids, const float* grad_logp, const float* grad_entropy,
+                                        void* grad, int64_t ldg, void* stream) {
   if (int rc = check_logits(logits, ldl, dtype, targets, rows, vocab)) return rc;
   SRA_REQUIRE(top >= 0 && top <= vocab, SRA_ERR_ARG, "top must be in [0, vocab], got %d", top);
   SRA_REQUIRE(top <= SRA_TOKEN_MAX_TOP, SRA_ERR_UNSUPPORTED, "top %d is above %d", top, SRA_TOKEN_MAX_TOP);
@@ -690,17 +713,26 @@ extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype
   if (grad != nullptr)
     if (int rc = check_grad(logits, ldl, grad, ldg, rows, vocab, dtype)) return rc;
   if (rows == 0) return SRA_OK;
-  const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, top, logp, entropy, lse, top_logp, top_ids,
-               grad_logp, grad_entropy, ldg};
+  const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, top, logp, entropy, lse, lse_rest, top_logp,
+               top_ids, grad_logp, grad_entropy, ldg};
   return with_type(dtype, [&](auto t) {
     return launch<decltype(t)>(logits, a, grad, static_cast<hipStream_t>(stream));
   });
 }
 
-extern "C" int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
-                                       int64_t rows, int64_t vocab, int64_t ignore, const float* lse,
-                                       const float* entropy, const float* grad_logp, const float* grad_entropy,
-                                       void* grad, int64_t ldg, void* stream) {
+extern "C" int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                  int64_t rows, int64_t vocab, int64_t ignore, int32_t top, float* logp,
+                                  float* entropy, float* lse, float* top_logp, int64_t* top_ids,
+                                  const float* grad_logp, const float* grad_entropy, void* grad, int64_t ldg,
+                                  void* stream) {
+  return sra_token_logprobs_split(logits, ldl, dtype, targets, rows, vocab, ignore, top, logp, entropy, lse, nullptr,
+                                  top_logp, top_ids, grad_logp, grad_entropy, grad, ldg, stream);
+}
+
+extern "C" int sra_token_logprobs_grad_split(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                             int64_t rows, int64_t vocab, int64_t ignore, const float* lse,
+                                             const float* lse_rest, const float* entropy, const float* grad_logp,
+                                             const float* grad_entropy, void* grad, int64_t ldg, void* stream) {
   if (int rc = check_logits(logits, ldl, dtype, targets, rows, vocab)) return rc;
   if (rows == 0) return SRA_OK;
   SRA_REQUIRE(lse != nullptr && grad_logp != nullptr && grad != nullptr, SRA_ERR_ARG,
@@ -709,13 +741,21 @@ extern "C" int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t 
               "grad_entropy needs the forward pass's entropy");
   if (int rc = check_grad(logits, ldl, grad, ldg, rows, vocab, dtype)) return rc;
   const Args a{ldl, targets, rows, static_cast<int>(vocab), ignore, 0, nullptr, nullptr, nullptr, nullptr, nullptr,
-               grad_logp, grad_entropy, ldg};
+               nullptr, grad_logp, grad_entropy, ldg};
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(cdiv(vocab, kGradSpan)));
     if (int rc = check_launch(rows, 256)) return rc;
     hipLaunchKernelGGL((logprob_grad_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T*>(logits), a, lse, entropy, static_cast<T*>(grad));
+                       static_cast<const T*>(logits), a, lse, lse_rest, entropy, static_cast<T*>(grad));
     return launch_status("logprob_grad_kernel");
   });
+}
+
+extern "C" int sra_token_logprobs_grad(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets,
+                                       int64_t rows, int64_t vocab, int64_t ignore, const float* lse,
+                                       const float* entropy, const float* grad_logp, const float* grad_entropy,
+                                       void* grad, int64_t ldg, void* stream) {
+  return sra_token_logprobs_grad_split(logits, ldl, dtype, targets, rows, vocab, ignore, lse, nullptr, entropy,
+                                       grad_logp, grad_entropy, grad, ldg, stream);
 }

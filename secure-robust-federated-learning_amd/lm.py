@@ -37,7 +37,12 @@ MAX_RANK = 64
 MAX_TOP = 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
-TokenLogprobs = namedtuple("TokenLogprobs", "logp entropy lse top_logp top_ids")
+
+class TokenLogprobs(namedtuple("TokenLogprobs", "logp entropy lse top_logp top_ids")):
+    """Beside the five: ``lse_rest``, what the rounding of lse left."""
+
+    lse_rest = None
+
 
 
 # ---------------------------------------------------------------------------
@@ -335,10 +340,11 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
         raise NotImplementedError("top %d is above %d" % (top, MAX_TOP))
 
     # logp, lse and the alternatives come as views of one buffer
-    f = torch.empty((2 + bool(entropy) + top) * R, dtype=torch.float32, device=dev)
-    rows = f[:(2 + bool(entropy)) * R].view(2 + bool(entropy), R).unbind(0)
-    res = TokenLogprobs(rows[0], rows[2] if entropy else None, rows[1], f[(2 + bool(entropy)) * R:].view(R, top),
+    f = torch.empty((3 + bool(entropy) + top) * R, dtype=torch.float32, device=dev)
+    rows = f[:(3 + bool(entropy)) * R].view(3 + bool(entropy), R).unbind(0)
+    res = TokenLogprobs(rows[0], rows[3] if entropy else None, rows[1], f[(3 + bool(entropy)) * R:].view(R, top),
                         torch.empty((R, top), dtype=torch.int64, device=dev))
+    res.lse_rest = rows[2]
     grad, ldg = None, 0
     if grad_logp is not None:
         grad_logp = _vector("grad_logp", grad_logp, R, torch.float32, dev)
@@ -349,9 +355,9 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
         if out is None:
             out = torch.empty((R, V), dtype=logits.dtype, device=dev)
         grad, ldg = _rows("out", out, (R, V), logits.dtype, dev, out=True)
-    _call(dev, "sra_token_logprobs", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V, int(ignore_index), top,
-          res.logp.data_ptr(), _ptr(res.entropy), res.lse.data_ptr(), res.top_logp.data_ptr(), res.top_ids.data_ptr(),
-          _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad), ldg)
+    _call(dev, "sra_token_logprobs_split", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V, int(ignore_index),
+          top, res.logp.data_ptr(), _ptr(res.entropy), res.lse.data_ptr(), res.lse_rest.data_ptr(),
+          res.top_logp.data_ptr(), res.top_ids.data_ptr(), _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad), ldg)
     return res, grad
 
 
@@ -363,7 +369,8 @@ def token_logprobs(logits, targets, top=0, entropy=False, ignore_index=-100):
     every row when asked, else None; lse the log of the sum of exponentials; the
     ``top`` <= 32 most probable tokens' log probabilities and ids, descending, the
     lowest id first among equals.  -inf logits have probability 0; a row of only
-    -inf, or with +inf or NaN, gives NaN."""
+    -inf (lse -inf), or with +inf or NaN, gives NaN.  ``lse_rest`` of the result is
+    what the rounding of lse left, for ``token_logprobs_grad``."""
     return _logprobs(logits, targets, top, entropy, ignore_index, None, None, None)[0]
 
 
@@ -379,14 +386,18 @@ def token_logprobs_and_grad(logits, targets, grad_logp, grad_entropy=None, top=0
     return _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entropy, out)
 
 
-def token_logprobs_grad(logits, targets, lse, grad_logp, entropy=None, grad_entropy=None, ignore_index=-100, out=None):
-    """The logits' gradient from a forward pass's lse (and entropy, which
-    grad_entropy needs).  ``out`` may be the logits (in place)."""
+def token_logprobs_grad(logits, targets, lse, grad_logp, entropy=None, grad_entropy=None, ignore_index=-100, out=None,
+                        lse_rest=None):
+    """The logits' gradient from a forward pass's lse and lse_rest (and entropy, which
+    grad_entropy needs).  Without lse_rest every probability of a row is off by up to
+    2^-24 |lse| of itself.  ``out`` may be the logits (in place)."""
     src = logits
     logits, ldl, code, targets = _logits(logits, targets)
     R, V = logits.shape
     dev = logits.device
     lse = _vector("lse", lse, R, torch.float32, dev)
+    if lse_rest is not None:
+        lse_rest = _vector("lse_rest", lse_rest, R, torch.float32, dev)
     grad_logp = _vector("grad_logp", grad_logp, R, torch.float32, dev)
     if grad_entropy is not None:
         if entropy is None:
@@ -398,8 +409,8 @@ def token_logprobs_grad(logits, targets, lse, grad_logp, entropy=None, grad_entr
     if out is None:
         out = torch.empty((R, V), dtype=logits.dtype, device=dev)
     out, ldg = _rows("out", out, (R, V), logits.dtype, dev, out=True)
-    _call(dev, "sra_token_logprobs_grad", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V, int(ignore_index),
-          lse.data_ptr(), _ptr(entropy), grad_logp.data_ptr(), _ptr(grad_entropy), out.data_ptr(), ldg)
+    _call(dev, "sra_token_logprobs_grad_split", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V,
+          int(ignore_index), lse.data_ptr(), _ptr(lse_rest), _ptr(entropy), grad_logp.data_ptr(), _ptr(grad_entropy), out.data_ptr(), ldg)
     return out
 
 
@@ -455,15 +466,15 @@ class _TokenLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index):
         res = token_logprobs(logits, targets, entropy=True, ignore_index=ignore_index)
-        ctx.save_for_backward(logits, targets, res.lse, res.entropy)
+        ctx.save_for_backward(logits, targets, res.lse, res.lse_rest, res.entropy)
         ctx.ignore_index = ignore_index
         return res.logp, res.entropy
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp, dent):
-        logits, targets, lse, ent = ctx.saved_tensors
-        return token_logprobs_grad(logits, targets, lse, dlogp, ent, dent, ctx.ignore_index), None, None
+        logits, targets, lse, rest, ent = ctx.saved_tensors
+        return token_logprobs_grad(logits, targets, lse, dlogp, ent, dent, ctx.ignore_index, lse_rest=rest), None, None
 
 
 def adapters(base, x, A, B, offsets, slots, scale=1.0):

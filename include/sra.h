@@ -475,7 +475,8 @@ int sra_bulyan_dba_f32(const float* X, int64_t n, int64_t d, int64_t ldx, int32_
  * slot slots[s] (device int32): the row of the clients' matrices it belongs
  * to, or -1 for none.  Two segments may share a slot.  Tokens that no segment
  * covers have no slot.  A slot outside [-1, nslots) or a token id outside the
- * vocabulary counts as none and is reported by sra_row_fault_count; offsets
+ * vocabulary counts as none and is reported by sra_row_fault_count, which each
+ * such token (or row of k14 with a bad target) raises by one a call; offsets
  * outside [0, tokens] are clamped.  A call that would need a launch of 2^32
  * threads or more is refused. */
 typedef enum { SRA_F32 = 0, SRA_BF16 = 1, SRA_F16 = 2 } sra_dtype;

@@ -292,6 +292,8 @@ __device__ __forceinline__ void mma(f32x4& acc, const Floats& a, const Floats& b
 // e_i / TT + i on: e_{i+1} / TT + i + 1 is never below the last of them.  A
 // workgroup finds its tile on the device by searching those numbers; the rows
 // before the first and behind the last segment count as segments without a slot.
+// The tokens of a bad slot are counted by the first launch of a call that finds
+// them, one workgroup a tile.
 // ---------------------------------------------------------------------------
 struct Segs {
   const int64_t* offsets;
@@ -311,7 +313,7 @@ __device__ __forceinline__ int seg_start(const Segs& sg, int i) {
 }
 
 template <int TT>
-__device__ __forceinline__ Tile find_tile(const Segs& sg, int tile) {
+__device__ __forceinline__ Tile find_tile(const Segs& sg, int tile, bool count_faults) {
   const int lane = threadIdx.x & 63, count = sg.nseg + 2;
   int lo, first, end, slot;
   if (count <= 256) {
@@ -360,7 +362,7 @@ __device__ __forceinline__ Tile find_tile(const Segs& sg, int tile) {
   t.n = t0 < first ? 0 : static_cast<int>(max(int64_t{0}, min(end - t0, int64_t{TT})));
   t.slot = slot;
   if (t.n > 0 && (slot < -1 || slot >= sg.nslots)) {
-    count_row_fault();
+    if (count_faults && threadIdx.x == 0) count_row_fault(t.n);
     t.slot = -1;
   }
   return t;
@@ -506,14 +508,14 @@ constexpr int shrink_cols() {
 template <typename T, typename W, int RT, int NT, bool AT>
 __global__ void __launch_bounds__(kThreads)
     shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, Segs sg, int width,
-                  int parts, int part, int rank, float* __restrict__ H) {
+                  int parts, int part, int rank, float* __restrict__ H, bool count_faults) {
   constexpr int KB = shrink_cols<T, W, RT, NT>(), PIECES = KB / 8;
   using SX = Stage<T, T, 16 * NT, PIECES, false, 1, true>;
   using SW = Stage<T, W, 16 * RT, PIECES, AT, AT ? 4 : 1, true>;
   __shared__ u32x4 lds[(SX::kBytes + SW::kBytes) / 16];
   u32x4* const ldw_ = lds + SX::kBytes / 16;
   const int tile = static_cast<int>(blockIdx.x) / parts, pt = static_cast<int>(blockIdx.x) % parts;
-  const Tile tl = find_tile<16 * NT>(sg, tile);
+  const Tile tl = find_tile<16 * NT>(sg, tile, count_faults && pt == 0);
   if (tl.n <= 0) return;
   float* Hp = H + (static_cast<int64_t>(pt) * sg.tokens + tl.t0) * rank;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -606,7 +608,7 @@ __global__ void __launch_bounds__(kThreads)
   using SW = Stage<T, W, COLS, RP, !AT, PC, false>;                 // RP pieces of 8 ranks
   __shared__ u32x4 lds[SW::kBytes / 16];
   const int tile = static_cast<int>(blockIdx.x) / blocks, block = static_cast<int>(blockIdx.x) % blocks;
-  const Tile tl = find_tile<16 * NT>(sg, tile);
+  const Tile tl = find_tile<16 * NT>(sg, tile, false);
   if (tl.n <= 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
@@ -896,9 +898,9 @@ __global__ void __launch_bounds__(256)
 template <typename T, typename W>
 __global__ void __launch_bounds__(256)
     tiny_shrink_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, int64_t ldw, int64_t si,
-                       int64_t sj, Segs sg, int width, int rank, float* __restrict__ H) {
+                       int64_t sj, Segs sg, int width, int rank, float* __restrict__ H, bool count_faults) {
   const int64_t t = blockIdx.x;
-  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t);
+  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t, count_faults && threadIdx.x == 0);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int i = wave; i < rank; i += 4) {
     float a = 0.f;
@@ -915,7 +917,7 @@ __global__ void __launch_bounds__(256)
     tiny_expand_kernel(const T* base, int64_t ldb, const float* __restrict__ H, const W* __restrict__ w, int64_t ldw,
                        int64_t si, int64_t sj, Segs sg, int width, int rank, float scale, T* out, int64_t ldo) {
   const int64_t t = blockIdx.x;
-  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t);
+  const int c = token_slot(sg.offsets, sg.slots, sg.nseg, sg.nslots, t, false);
   for (int j = threadIdx.x; j < width; j += 256) {
     const float b = base != nullptr ? to_f32(base[t * ldb + j]) : 0.f;
     float a = 0.f;
@@ -953,6 +955,15 @@ __global__ void __launch_bounds__(256)
   float* g = G + c * ldg + i * si + j * sj;
   if (!accumulate) *g = scale * a;
   else if (any) *g += scale * a;
+}
+
+// the tokens of bad slots, for a gradient of B alone from given hidden values: no
+// tile is searched for there
+__global__ void __launch_bounds__(256) count_slots_kernel(Segs sg) {
+  for (int i = threadIdx.x; i < sg.nseg; i += 256) {
+    const int c = sg.slots[i], n = seg_start(sg, i + 2) - seg_start(sg, i + 1);
+    if (n > 0 && (c < -1 || c >= sg.nslots)) count_row_fault(n);
+  }
 }
 
 struct Shape {
@@ -1054,12 +1065,12 @@ static int with_tile(const Segs& sg, int rank, F&& f) {
 
 template <typename T, typename W, bool AT>
 static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw, const Segs& sg, int64_t width,
-                         int parts, int rank, float* H, hipStream_t st) {
+                         int parts, int rank, float* H, bool count_faults, hipStream_t st) {
   if (width < 8) {
     if (int rc = check_launch(sg.tokens, 256)) return rc;
     hipLaunchKernelGGL((tiny_shrink_kernel<T, W>), dim3(static_cast<unsigned>(sg.tokens)), dim3(256), 0, st,
                        static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, AT ? 1 : width,
-                       AT ? static_cast<int64_t>(rank) : 1, sg, static_cast<int>(width), rank, H);
+                       AT ? static_cast<int64_t>(rank) : 1, sg, static_cast<int>(width), rank, H, count_faults);
     return launch_status("tiny_shrink_kernel");
   }
   return with_tile(sg, rank, [&](auto nt, auto rt) {
@@ -1068,7 +1079,7 @@ static int launch_shrink(const void* x, int64_t ldx, const void* w, int64_t ldw,
     if (int rc = check_launch(static_cast<int64_t>(tile_count<16 * NT>(sg)) * parts, kThreads)) return rc;
     hipLaunchKernelGGL((shrink_kernel<T, W, RT, NT, AT>), dim3(tile_count<16 * NT>(sg) * parts), dim3(kThreads), 0, st,
                        static_cast<const T*>(x), ldx, static_cast<const W*>(w), ldw, sg, static_cast<int>(width),
-                       parts, part, rank, H);
+                       parts, part, rank, H, count_faults);
     return launch_status("shrink_kernel");
   });
 }
@@ -1162,7 +1173,7 @@ static int run_apply(const void* base, int64_t ldbase, const void* x, int64_t ld
                      const Shape& sh, void* out, int64_t ldo, float* hidden, char* ws, hipStream_t st) {
   const int parts = shrink_parts(sg.tokens, sg.nseg, sh.k, sh.rank);
   float* H = reinterpret_cast<float*>(ws);
-  if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, parts, sh.rank, H, st)) return rc;
+  if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, parts, sh.rank, H, true, st)) return rc;
   return launch_expand<T, W, true>(base, ldbase, H, parts, w.B, w.ldb, sg, sh.m, sh.rank, sh.scale, out, ldo,
                                    hidden, st);
 }
@@ -1192,15 +1203,19 @@ static int run_grad(const void* dout, int64_t lddo, const void* x, int64_t ldx, 
       const int parts = g.dx != nullptr ? shrink_parts(sg.tokens, sg.nseg, sh.m, sh.rank) : 1;
       float* Zp = Z;
       if (parts > 1) Z = Zp + static_cast<int64_t>(parts) * sg.tokens * sh.rank;
-      if (int rc = launch_shrink<T, W, true>(dout, lddo, w.B, w.ldb, sg, sh.m, parts, sh.rank, Zp, st)) return rc;
+      if (int rc = launch_shrink<T, W, true>(dout, lddo, w.B, w.ldb, sg, sh.m, parts, sh.rank, Zp, true, st)) return rc;
       if (g.dx != nullptr)
         if (int rc = launch_expand<T, W, false>(g.dxbase, g.lddxb, Zp, parts, w.A, w.lda, sg, sh.k, sh.rank, sh.scale,
                                                 g.dx, g.lddx, parts > 1 ? Z : nullptr, st))
           return rc;
     }
+    const bool counted = g.dx != nullptr || g.dA != nullptr;
     if (g.dB != nullptr && H == nullptr) {
       H = Hw;
-      if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, 1, sh.rank, Hw, st)) return rc;
+      if (int rc = launch_shrink<T, W, false>(x, ldx, w.A, w.lda, sg, sh.k, 1, sh.rank, Hw, !counted, st)) return rc;
+    } else if (!counted) {
+      hipLaunchKernelGGL(count_slots_kernel, dim3(1), dim3(256), 0, st, sg);
+      if (int rc = launch_status("count_slots_kernel")) return rc;
     }
   }
   if (g.dA != nullptr)

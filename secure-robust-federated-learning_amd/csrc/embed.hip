@@ -24,7 +24,7 @@ struct Tokens {
 // row of the (nslots * vocab, dim) table that token t reads, -1 for none; one
 // caller a token counts its fault
 __device__ __forceinline__ int64_t token_row(const Tokens& k, int64_t t, int& slot, int64_t& id, bool count) {
-  slot = token_slot(k.offsets, k.slots, k.nseg, k.nslots, t);
+  slot = token_slot(k.offsets, k.slots, k.nseg, k.nslots, t, count);
   id = k.ids[t];
   if (slot < 0) return -1;
   if (id < 0 || id >= k.vocab) {

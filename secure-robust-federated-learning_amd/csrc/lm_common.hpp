@@ -20,19 +20,20 @@ __device__ __forceinline__ T from_f32(float v) {
   return static_cast<T>(v);
 }
 
-__device__ __forceinline__ void count_row_fault() {
+// of `tokens` tokens; called by one lane for them
+__device__ __forceinline__ void count_row_fault(unsigned tokens = 1) {
 #ifdef SRA_DEVICE_ASSERT
   __builtin_trap();
 #else
-  atomicAdd(&g_row_faults, 1u);
+  atomicAdd(&g_row_faults, tokens);
 #endif
 }
 
-// slots[s] for a segment that holds tokens, checked: -1 for none.
-__device__ __forceinline__ int checked_slot(const int32_t* __restrict__ slots, int s, int nslots) {
+// slots[s] for a token of segment s, checked: -1 for none.
+__device__ __forceinline__ int checked_slot(const int32_t* __restrict__ slots, int s, int nslots, bool count) {
   const int c = slots[s];
   if (c < -1 || c >= nslots) {
-    count_row_fault();
+    if (count) count_row_fault();
     return -1;
   }
   return c;
@@ -49,13 +50,14 @@ __device__ __forceinline__ int segment_of(const int64_t* __restrict__ offsets, i
   return lo;
 }
 
-// Slot of token t, -1 for none (no covering segment, slot -1, or a bad slot).
+// Slot of token t, -1 for none (no covering segment, slot -1, or a bad slot); one
+// caller a token and call counts its fault.
 __device__ __forceinline__ int token_slot(const int64_t* __restrict__ offsets, const int32_t* __restrict__ slots,
-                                          int nseg, int nslots, int64_t t) {
+                                          int nseg, int nslots, int64_t t, bool count) {
   if (offsets == nullptr) return 0;
   const int s = segment_of(offsets, nseg, t);
   if (s < 0 || t >= offsets[s + 1]) return -1;
-  return checked_slot(slots, s, nslots);
+  return checked_slot(slots, s, nslots, count);
 }
 
 inline int dtype_size(int32_t dtype) { return dtype == SRA_F32 ? 4 : 2; }

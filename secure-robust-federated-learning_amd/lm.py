@@ -18,8 +18,8 @@ the clients' (N, D) matrices (``store.ClientBank``):
 tensors: tokens [offsets[s], offsets[s + 1]) belong to row ``slots[s]`` of the
 clients' matrices, -1 for none; tokens no segment covers have none either.  They
 are read on the device only, so a captured graph replays with new values.  A
-slot or token id outside its range is treated as none and counted
-(``engine.row_fault_count``).
+slot or token id outside its range is treated as none and counted, once a token
+and call (``engine.row_fault_count``).
 
 Everything runs on torch's current stream of the tensors' device and allocates
 through torch's caching allocator.  There is no CPU path.

@@ -492,7 +492,8 @@ typedef enum { SRA_F32 = 0, SRA_BF16 = 1, SRA_F16 = 2 } sra_dtype;
  * and out_t = base_t where t has no slot.  x, base and out have dtype; base
  * may be NULL (zeros) or equal out (in place, same row stride).  hidden
  * (optional, tokens x rank float32) receives h (0 without a slot).  Sums are
- * float32.  1 <= rank <= SRA_ADAPTER_MAX_RANK. */
+ * float32; products with an infinite operand come out infinite or NaN, and so may
+ * sums within 2^-8 of float32's largest value.  1 <= rank <= SRA_ADAPTER_MAX_RANK. */
 int sra_adapter_workspace_bytes(int64_t tokens, int32_t nseg, int32_t nslots, int64_t k, int64_t m, int32_t rank,
                                 size_t* bytes);
 int sra_adapter_apply(const void* base, int64_t ldbase, const void* x, int64_t ldx, const void* A, int64_t lda,

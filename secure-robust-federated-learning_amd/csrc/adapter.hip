@@ -17,8 +17,9 @@
 // below 2^-16 (or 2^-8) of the whole are left out.  Memory bounds all three
 // products, so the matrix instructions, up to five for one, have room.  A product
 // with an infinity is then the sum of several that may have opposite signs: it
-// comes out infinite or NaN.  float32 activations run on the float32 units
-// (v_mfma_f32_16x16x4_f32).
+// comes out infinite or NaN.  A finite one keeps its digits up to float32's largest
+// value, but sums within 2^-8 of that may pass it on their way.  float32
+// activations run on the float32 units (v_mfma_f32_16x16x4_f32).
 //
 // Layout.  A lane (n = lane % 16, g = lane / 16) of a 16x16 product holds row or
 // column n of its operands with the inner indices g * 8 .. g * 8 + 7 and, of the
@@ -191,18 +192,26 @@ template <typename T, typename S, bool FULL = false>
 using Frag = std::conditional_t<std::is_same_v<T, float>, Floats,
                                 Terms<std::is_same_v<S, __bf16> ? 1 : std::is_same_v<S, float> && FULL ? 3 : 2>>;
 
-// values e and e + 1, e even: the nearest bf16, that of the rest, that of its rest
-template <int N>
+// values e and e + 1, e even, of type S: the nearest bf16, that of the rest, that of
+// its rest.  A float32 above bf16's largest value, whose nearest bf16 is infinite,
+// has that largest one as its first term.
+constexpr float kMostBf16 = 3.3895314e38f;
+template <typename S, int N>
 __device__ __forceinline__ void put2(Terms<N>& f, int e, f32x2 x) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    f.t[i][e / 2] = pack2<__bf16>(x[0], x[1]);
+    if (std::is_same_v<S, float> && i == 0)
+      f.t[i][e / 2] = pack2<__bf16>(__builtin_amdgcn_fmed3f(x[0], -kMostBf16, kMostBf16),
+                                    __builtin_amdgcn_fmed3f(x[1], -kMostBf16, kMostBf16));
+    else
+      f.t[i][e / 2] = pack2<__bf16>(x[0], x[1]);
     if (i + 1 < N) {
       const f32x2 h = unpack2<__bf16>(f.t[i][e / 2]);
       x = f32x2{x[0] - h[0], x[1] - h[1]};
     }
   }
 }
+template <typename S>
 __device__ __forceinline__ void put2(Floats& f, int e, f32x2 x) {
   f.v[e] = x[0];
   f.v[e + 1] = x[1];
@@ -216,7 +225,7 @@ __device__ __forceinline__ F frag_of(const Raw8<S>& r) {
     for (int b = 0; b < 4; ++b) f.t[0][b] = r.w[b];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) put2(f, e, r.get2(e));
+    for (int e = 0; e < 8; e += 2) put2<S>(f, e, r.get2(e));
   }
   return f;
 }
@@ -230,7 +239,7 @@ __device__ __forceinline__ F column_of(const RawN<S, N> (&r)[8], int a) {
     if constexpr (std::is_same_v<S, __bf16>)
       f.t[0][e / 2] = __builtin_amdgcn_perm(r[e + 1].w[a / 2], r[e].w[a / 2], a % 2 ? 0x07060302u : 0x05040100u);
     else
-      put2(f, e, f32x2{to_f32(r[e].get(a)), to_f32(r[e + 1].get(a))});
+      put2<S>(f, e, f32x2{to_f32(r[e].get(a)), to_f32(r[e + 1].get(a))});
   }
   return f;
 }
@@ -660,7 +669,7 @@ __global__ void __launch_bounds__(kThreads)
           if (i + e < rank) Hsum[at + i + e] = h[e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) put2(fh[b], e, f32x2{h[e] * scale, h[e + 1] * scale});
+    for (int e = 0; e < 8; e += 2) put2<float>(fh[b], e, f32x2{h[e] * scale, h[e + 1] * scale});
   }
   const int row = (NT == 1 ? wave * 64 : 0) + n * PC;    // this lane's columns of a stage
   auto base_at = [&](int q, int j0) { return (tl.t0 + min(tok + g * 4 + q, tl.n - 1)) * ldb + j0 + row; };

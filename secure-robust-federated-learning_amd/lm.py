@@ -22,7 +22,9 @@ slot or token id outside its range is treated as none and counted, once a token
 and call (``engine.row_fault_count``).
 
 Everything runs on torch's current stream of the tensors' device and allocates
-through torch's caching allocator.  There is no CPU path.
+through torch's caching allocator.  Tensors given to be written (``out`` and the
+like) get a new version, as torch's own in-place operations give.  There is no CPU
+path.
 """
 from __future__ import annotations
 
@@ -134,6 +136,11 @@ def _call(device, name, *args):
             _lib.call(name, *args, _raw_stream(index))
 
 
+# The kernels write behind torch's back: the caller's tensors get a new version, so
+# that autograd refuses a backward pass through what it saved before.
+_written = torch.autograd.graph.increment_version
+
+
 @functools.lru_cache(maxsize=4096)
 def _bytes(name, *args):
     """A workspace size: a function of the sizes alone."""
@@ -189,7 +196,8 @@ def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=Fal
     if base is not None:
         base, ldbase = _rows("base", base, (T, M), x.dtype, dev)
     ldo = M
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((T, M), dtype=x.dtype, device=dev)
     else:
         out, ldo = _rows("out", out, (T, M), x.dtype, dev, out=True)
@@ -197,6 +205,8 @@ def adapter_apply(base, x, A, B, offsets, slots, scale=1.0, out=None, hidden=Fal
     ws, nb = _adapter_workspace(T, slots.shape[0], n, K, M, r, dev)
     _call(dev, "sra_adapter_apply", _ptr(base), ldbase, *head, float(scale), dtype, wdtype, out.data_ptr(), ldo,
           _ptr(H), ws.data_ptr(), nb)
+    if given:
+        _written(out)
     return (out, H) if hidden else out
 
 
@@ -238,6 +248,9 @@ def adapter_grad(grad_out, x, A, B, offsets, slots, scale=1.0, hidden=None, base
     _call(dev, "sra_adapter_grad", dy.data_ptr(), lddy, *head, float(scale), dtype, wdtype, _ptr(hidden),
           _ptr(base_grad), lddxb, _ptr(dx), lddx, _ptr(dA), ldda, _ptr(dB), lddb, int(bool(accumulate)),
           ws.data_ptr(), nb)
+    for asked, t in ((grad_x, dx), (grad_A, dA), (grad_B, dB)):
+        if t is not None and asked is not True:
+            _written(t)
     return dx, dA, dB
 
 
@@ -277,13 +290,16 @@ def embed(table, ids, offsets=None, slots=None, scale=1.0, dtype=None, out=None)
     dev = full.device
     ids = _vector("ids", _device_tensor("ids", ids, dev), ids.numel(), torch.int64, dev)
     T = ids.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((T, E), dtype=dtype or full.dtype, device=dev)
     elif dtype is not None and out.dtype != dtype:
         raise TypeError("out must be %s, got %s" % (dtype, out.dtype))
     out, ldo = _rows("out", out, (T, E), None, dev, out=True)
     _call(dev, "sra_embed", full.data_ptr(), ld, code, ids.data_ptr(), _ptr(off), _ptr(sl), S, T, n, V, E,
           float(scale), out.data_ptr(), ldo, _float_code("out", out))
+    if given:
+        _written(out)
     return out
 
 
@@ -312,6 +328,7 @@ def embed_grad(grad_out, ids, grad, offsets=None, slots=None, scale=1.0, padding
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
     _call(dev, "sra_embed_grad", dy.data_ptr(), lddy, code, ids.data_ptr(), _ptr(off), _ptr(sl), S, T, n, V, E,
           float(scale), pad, full.data_ptr(), ld, int(bool(accumulate)), ws.data_ptr(), nb)
+    _written(grad)
     return grad
 
 
@@ -345,7 +362,7 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
     res = TokenLogprobs(rows[0], rows[3] if entropy else None, rows[1], f[(3 + bool(entropy)) * R:].view(R, top),
                         torch.empty((R, top), dtype=torch.int64, device=dev))
     res.lse_rest = rows[2]
-    grad, ldg = None, 0
+    grad, ldg, given = None, 0, out is not None
     if grad_logp is not None:
         grad_logp = _vector("grad_logp", grad_logp, R, torch.float32, dev)
         if grad_entropy is not None:
@@ -358,6 +375,8 @@ def _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entro
     _call(dev, "sra_token_logprobs_split", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V, int(ignore_index),
           top, res.logp.data_ptr(), _ptr(res.entropy), res.lse.data_ptr(), res.lse_rest.data_ptr(),
           res.top_logp.data_ptr(), res.top_ids.data_ptr(), _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad), ldg)
+    if given:
+        _written(grad)
     return res, grad
 
 
@@ -406,11 +425,14 @@ def token_logprobs_grad(logits, targets, lse, grad_logp, entropy=None, grad_entr
         entropy = _vector("entropy", entropy, R, torch.float32, dev)
     if out is src and logits is not src:
         raise ValueError("out can be the logits only where they have unit column stride")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((R, V), dtype=logits.dtype, device=dev)
     out, ldg = _rows("out", out, (R, V), logits.dtype, dev, out=True)
     _call(dev, "sra_token_logprobs_grad_split", logits.data_ptr(), ldl, code, targets.data_ptr(), R, V,
           int(ignore_index), lse.data_ptr(), _ptr(lse_rest), _ptr(entropy), grad_logp.data_ptr(), _ptr(grad_entropy), out.data_ptr(), ldg)
+    if given:
+        _written(out)
     return out
 
 

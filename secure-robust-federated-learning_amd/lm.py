@@ -123,7 +123,8 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# absent from a torch without GPU support, whose tensors are refused before it is needed
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _call(device, name, *args):

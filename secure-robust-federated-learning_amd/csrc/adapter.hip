@@ -1138,10 +1138,20 @@ static int launch_expand(const void* base, int64_t ldb, const float* H, int part
   });
 }
 
+// whether a gradient of so many tokens is summed element by element
+static bool outer_tiny(int64_t tokens, int64_t width, int rank) { return width < 8 || tokens * rank < 8; }
+
+// the largest of launch_outer's grids, which go by the weight's size alone where
+// there are no tokens
+static int check_outer(const Segs& sg, int64_t width, int rank) {
+  const int64_t per = rank * width;
+  return check_launch(outer_tiny(sg.tokens, width, rank) ? cdiv(per, 256) : cdiv(per, 1024), 256);
+}
+
 template <typename T, bool AT>
 static int launch_outer(const void* x, int64_t ldx, const float* H, const Segs& sg, int64_t width, int rank,
                         float scale, float* G, int64_t ldg, int accumulate, float* parts_ws, hipStream_t st) {
-  if (width < 8 || sg.tokens * rank < 8) {
+  if (outer_tiny(sg.tokens, width, rank)) {
     const dim3 tg(static_cast<unsigned>(cdiv(rank * width, 256)), static_cast<unsigned>(sg.nslots));
     hipLaunchKernelGGL((tiny_outer_kernel<T>), tg, dim3(256), 0, st, static_cast<const T*>(x), ldx, H, sg,
                        static_cast<int>(width), rank, scale, G, ldg, AT ? 1 : width,
@@ -1313,6 +1323,10 @@ extern "C" int sra_adapter_grad(const void* dout, int64_t lddo, const void* x, i
   SRA_REQUIRE(ws != nullptr && ws_bytes >= need, SRA_ERR_WORKSPACE, "adapter workspace: need %zu bytes, got %zu", need,
               ws_bytes);
   SRA_REQUIRE(dx == nullptr || (dx != dout && dx != x), SRA_ERR_ARG, "dx must not be dout or x: they are read after it");
+  if (dA != nullptr)
+    if (int rc = check_outer(sg, k, rank)) return rc;
+  if (dB != nullptr)
+    if (int rc = check_outer(sg, m, rank)) return rc;
   const GradOut g{hidden, dxbase, lddxb, dx, lddx, dA, ldda, dB, lddb, accumulate};
   const Weights wt{A, lda, B, ldb};
   return with_types(dtype, wdtype, [&](auto t, auto w) {

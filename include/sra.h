@@ -522,7 +522,7 @@ int sra_adapter_grad(const void* dout, int64_t lddo, const void* x, int64_t ldx,
 /* k13: embedding lookup with scaling.  Slot c's table (vocab x dim, row-major,
  * tdtype) starts at table + c * ldt; offsets = slots = NULL reads slot 0 for
  * every token.  out_t = scale * table_c[ids[t]] rounded once to odtype; zeros
- * for a token without a slot. */
+ * for a token without a slot.  out must not be the table. */
 int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const int64_t* ids, const int64_t* offsets,
               const int32_t* slots, int32_t nseg, int64_t tokens, int32_t nslots, int64_t vocab, int64_t dim,
               float scale, void* out, int64_t ldo, int32_t odtype, void* stream);
@@ -531,8 +531,8 @@ int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const int64_t* ids
  * tokens t of slot c with ids[t] = v, t ascending, in float32; grad is float32
  * with slot stride ldg.  Tokens with ids[t] = padding (pass -1 for none) are
  * left out.  Every row is written, zeros where no token reads it; accumulate
- * != 0 adds to the rows that tokens read and leaves the others alone.
- * nslots * vocab < 2^32 - 1, tokens < 2^31. */
+ * != 0 adds to the rows that tokens read and leaves the others alone.  grad must
+ * not be dout.  nslots * vocab < 2^32 - 1, tokens < 2^31. */
 int sra_embed_grad_workspace_bytes(int64_t tokens, int64_t dim, size_t* bytes);
 int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t* ids, const int64_t* offsets,
                    const int32_t* slots, int32_t nseg, int64_t tokens, int32_t nslots, int64_t vocab, int64_t dim,

@@ -455,7 +455,7 @@ extern "C" int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const i
   SRA_REQUIRE(tokens <= 1 || ldo >= dim, SRA_ERR_SHAPE, "out needs a row stride >= dim");
   if (tokens == 0) return SRA_OK;
   return with_type(tdtype, [&](auto w) {
-    return with_type(odtype, [&](auto t) {
+    return with_type(odtype, [&](auto t) -> int {
       using W = decltype(w);
       using T = decltype(t);
       // 16 lanes a token unless that leaves the card less than 4 waves a compute unit
@@ -464,6 +464,7 @@ extern "C" int sra_embed(const void* table, int64_t ldt, int32_t tdtype, const i
       const bool few = tokens * 16 < 64 * 1024;
       const int64_t blocks = cdiv(tokens * (few ? 64 : 16), 256);
       if (int rc = check_launch(blocks, 256)) return rc;
+      SRA_REQUIRE(out != table, SRA_ERR_ARG, "out must not be the table: other tokens read it");
       const dim3 grid(static_cast<unsigned>(blocks));
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const W*>(table),
@@ -519,6 +520,7 @@ extern "C" int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, con
   const int window = window_of(tokens, dim);
   const int64_t units = cdiv(tokens, window) * chunks;
   if (int rc = check_launch(cdiv(units, 4), 256)) return rc;
+  SRA_REQUIRE(tokens == 0 || dout != grad, SRA_ERR_ARG, "grad must not be dout: it is written before dout is read");
   // the passes end in `sorted`
   int passes = 0;
   for (int64_t run = kTile; run < tokens; run *= kGroup) ++passes;

@@ -285,7 +285,7 @@ def embed(table, ids, offsets=None, slots=None, scale=1.0, dtype=None, out=None)
 
     The product is formed in float32 and rounded once to ``dtype`` (the table's by
     default).  ids (T,) are int64.  Tokens without a slot, or with an id outside
-    the vocabulary (counted), get zeros."""
+    the vocabulary (counted), get zeros.  ``out`` must not be the table."""
     full, ld, n, V, E, (off, sl, S) = _table("table", table, offsets, slots)
     code = _float_code("table", full)
     dev = full.device
@@ -311,7 +311,7 @@ def embed_grad(grad_out, ids, grad, offsets=None, slots=None, scale=1.0, padding
 
     Tokens with ids[t] = padding_idx add nothing.  Every row is written, zeros
     where no token reads it; accumulate=True adds to the rows that tokens read and
-    leaves the others alone."""
+    leaves the others alone.  ``grad`` must not be grad_out."""
     full, ld, n, V, E, (off, sl, S) = _table("grad", grad, offsets, slots, out=True)
     dev = full.device
     if full.dtype != torch.float32:

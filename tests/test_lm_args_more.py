@@ -22,3 +22,18 @@ def test_gradients_of_an_empty_batch_too_large_for_a_launch(which):
     a.update({which: P, "ldd" + which[1]: r * k})
     with pytest.raises(NotImplementedError, match="too many"):
         _lib.call("sra_adapter_grad", *a.values(), None)
+
+
+def test_embedding_gradient_over_the_gradient_it_reads():
+    """The gradient is cleared before the tokens' gradients are read."""
+    a = dict(dout=P, lddo=8, dtype=0, ids=Q, offsets=None, slots=None, nseg=0, tokens=64, nslots=1, vocab=64, dim=8,
+             scale=1.0, padding=-1, grad=P, ldg=512, accumulate=0, ws=Q, ws_bytes=BIG)
+    with pytest.raises(ValueError, match="grad must not be dout"):
+        _lib.call("sra_embed_grad", *a.values(), None)
+
+
+def test_lookup_over_its_table():
+    a = dict(table=P, ldt=512, tdtype=0, ids=Q, offsets=None, slots=None, nseg=0, tokens=64, nslots=1, vocab=64, dim=8,
+             scale=1.0, out=P, ldo=8, odtype=0)
+    with pytest.raises(ValueError, match="out must not be the table"):
+        _lib.call("sra_embed", *a.values(), None)

@@ -225,6 +225,7 @@ class ClientBank:
             raise RuntimeError("load the round's choices before recording")
         for i, c in enumerate(self.choices):
             self.store._record(c, (self._ptrs.data_ptr() + 8 * i, self._seg.data_ptr(), 1, self.store.D))
+        torch.autograd.graph.increment_version(self.P)      # written through its address
 
 
 def fl_round(network, store, choices, local_update, args, state=None, attack="noattack", mal_index=(), bank=None):

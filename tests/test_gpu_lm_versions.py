@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import srfl_amd.lm as lm
+import srfl_amd.store as store
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,20 @@ def test_inference_tensors_have_none():
         out = torch.empty(T, 24, device="cuda")
         lm.adapter_apply(None, rand(T, 16), rand(1, 2, 16), rand(1, 24, 2), o, s, out=out)
     assert torch.isfinite(out).all()
+
+
+def test_a_bank_that_records():
+    """Its rows go back to the snapshot."""
+    params = [rand(5, 4), rand(3)]
+    S = store.ClientStore(params, 3)
+    S.snapshot()
+    bank = store.ClientBank(S, 2)
+    bank.load([2, 0])
+    bank.G.fill_(1.0)
+    bank.step(0.5)
+    w = rand(2, 5, 4).requires_grad_()
+    loss = (bank.param(0) * w).sum()                         # saves the rows
+    bank.record()
+    assert torch.equal(bank.param(0)[0], params[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

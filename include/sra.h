@@ -555,7 +555,8 @@ int sra_embed_grad(const void* dout, int64_t lddo, int32_t dtype, const int64_t*
  * writes the logits' gradient for given row gradients of logp and entropy:
  *   grad_i = grad_logp * (1[i = target] - p_i) - grad_entropy * p_i (log p_i + entropy)
  * (no logp part for an ignored or bad target; grad_entropy may be NULL), which
- * reads the logits from memory once for both.  A row whose parts are all absent
+ * reads the logits from memory once for both up to a vocabulary of 65536 (SRA_F32:
+ * 32768), twice beyond.  A row whose parts are all absent
  * or have the factor 0 gets zeros, whatever its logits are. */
 int sra_token_logprobs(const void* logits, int64_t ldl, int32_t dtype, const int64_t* targets, int64_t rows,
                        int64_t vocab, int64_t ignore, int32_t top, float* logp, float* entropy, float* lse,

@@ -498,8 +498,8 @@ struct Stage {
 // where the weight is the traffic): the waves share the stage's columns and their
 // sums meet in LDS in a fixed order.  W is [i][j] (AT false) or [j][i].
 // Bound by the read of x and W, in practice by waits at the stages' barriers:
-// bf16, rank 16, 8192 x 4096 18.5 us (4.1 TB/s); rank 64, 16384 x 8192 136 us
-// (2.2 TB/s), 175 us with W as [j][i], turned in registers.
+// bf16, rank 16, 8192 x 4096 19-20 us (3.8 TB/s); rank 64, 16384 x 8192 120 us
+// (2.5 TB/s), 152 us with W as [j][i], turned in registers.
 // ---------------------------------------------------------------------------
 // Columns a stage: fewer where three terms of the weight take LDS and registers
 // from a second and third workgroup of the compute unit (bf16 activations, float32
@@ -602,8 +602,8 @@ __global__ void __launch_bounds__(kThreads)
 // Neighbouring workgroups take the column blocks of one tile: between them they
 // read whole rows, not the same columns of many.  H comes in `parts` partial
 // sums; the first column block also writes their sum to Hsum when that is asked.
-// Bound by base and out: bf16, rank 16, 8192 x 4096 32 us (4.4 TB/s); rank 64,
-// 16384 x 8192 165-173 us (3.4 TB/s).
+// Bound by base and out: bf16, rank 16, 8192 x 4096 32-38 us (3.7-4.4 TB/s); rank
+// 64, 16384 x 8192 151-155 us (3.7 TB/s).
 // ---------------------------------------------------------------------------
 template <int NT>
 constexpr int kExpandCols = NT == 1 ? 256 : 128;
@@ -726,8 +726,11 @@ __global__ void __launch_bounds__(kThreads)
 // workgroups where there are few.  With one part the sums go to G ([i][j], or
 // [j][i] with AT), else each part's to its own copy (slot stride rank * width)
 // for join_parts.  Bound by the read of x; 190-250 registers a lane leave two waves
-// a SIMD: bf16, rank 64, 16384 x 8192 of 16 slots in 2 parts 150 us (2.4 TB/s);
-// stages of 64 tokens 185 us.
+// a SIMD: bf16, rank 64, 16384 x 8192 of 16 slots in 2 parts 141-152 us (2.4 TB/s);
+// stages of 64 tokens 185 us.  A slot's segments are walked one after another, and
+// the parts go by the average of tokens a slot: 16384 tokens of 4 clients in 4
+// segments 31 us, in 512 152 us, in 8192 2.3 ms; 6400 tokens of 100 clients 88 us for
+// the whole backward pass, 255 us where one of them has half.
 // ---------------------------------------------------------------------------
 constexpr int kOuterTokens = 128;
 constexpr int kOuterCols = 4;
@@ -869,7 +872,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // G_c = scale * sum of the parts, in order; 4 values a thread (two parts of 33.5
-// MB: 21 us, 4.8 TB/s)
+// MB: 21 us, 4.8 TB/s).  With accumulate every thread looks through the segments for
+// one of its slot (512 segments: 60 us more; 8192: 0.85 ms more).
 __global__ void __launch_bounds__(256)
     join_parts_kernel(const float* __restrict__ P, int parts, int64_t part_stride, Segs sg, int64_t per, float scale,
                       float* __restrict__ G, int64_t ldg, int accumulate) {

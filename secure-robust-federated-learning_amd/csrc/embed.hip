@@ -84,7 +84,8 @@ __device__ __forceinline__ void store8(S* p, const float (&x)[8]) {
 // Lookup: LANES lanes a token, 8 values a lane and step.  Bound by memory (a
 // read of the row, a write of the output); 16 lanes keep every lane busy at odd
 // widths, 64 spread few tokens over more waves.  32768 tokens, 2048 float32 values
-// to bf16: 60 us (6.7 TB/s, common rows from the caches).
+// to bf16: 59 us for 81 MB of different rows, some of them fetched by several dies
+// (150 MB in all), and 134 MB written: 4.8 TB/s.
 template <typename W, typename T, int LANES>
 __global__ void __launch_bounds__(256) embed_kernel(const W* __restrict__ table, int64_t ldt, Tokens k, float scale,
                                                     T* __restrict__ out, int64_t ldo) {
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const W* __restrict__ table,
 // place in its own run plus the count of smaller ones in the partner run, each
 // thread's 4 searches in step.  The same launch clears the gradient with the
 // workgroups behind the sorting ones: the sort hides behind that write (32768
-// tokens and 410 MB: 58 us, 7.1 TB/s).
+// tokens and 410 MB: 56 us, 7.3 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kTile = 4096;
 constexpr int kSortThreads = 1024;
@@ -237,8 +238,11 @@ __global__ void __launch_bounds__(256) merge_runs_kernel(const uint64_t* __restr
 // Sum: a wave takes a window of sorted positions and 512 columns, 8 rows' loads in
 // flight.  Runs that lie inside the window go to their row; a run that the window
 // shares with the one before (head) or after (tail) leaves a partial sum.  The window
-// where such a run starts then adds up the partials in order.  Bound by the gather
-// of dout's rows: 32768 x 2048 bf16 76 us, the join 16 us.
+// where such a run starts then adds up the partials in order, one wave for 512
+// columns: a run of most of a large batch (padding ids that padding_idx does not
+// leave out) is bound by that (2^20 tokens x 512 bf16: spread over 50001 rows 0.90
+// ms, half of them one id 3.3 ms, all of them 5.4 ms; left out by padding_idx 0.30).
+// Bound by the gather of dout's rows: 32768 x 2048 bf16 75 us, the join 15 us.
 // ---------------------------------------------------------------------------
 constexpr int kBatch = 8;
 constexpr int kCols = 512;
@@ -248,8 +252,9 @@ __device__ __forceinline__ unsigned row_at(const uint64_t* __restrict__ sorted, 
 }
 
 // Positions a window: 32 (a partial sum for 32 rows read), fewer where the waves
-// would not fill the card (32768 x 2048 104 us, 127 us with 8; 2000 x 512 35 us, 63
-// us with 32; sort and join included).
+// would not fill the card.  Added to a gradient, so without the clear, but with sort,
+// merge and join, common ids first: 32768 x 2048 of 50001 rows 138 us, 162 us with 8;
+// 2000 x 512 of 4001 36 us, 65 us with 32.
 static int window_of(int64_t tokens, int64_t dim) {
   int w = 32;
   while (w > 8 && cdiv(tokens, w) * cdiv(dim, kCols) < 4096) w /= 2;

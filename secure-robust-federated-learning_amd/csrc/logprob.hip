@@ -330,7 +330,7 @@ __device__ __forceinline__ void walk_tail(const T* row, int n, const Span& sp, i
 
 // The whole row, G stretches of a wave at a time: f(x[G][8], first index, step
 // between stretches, valid).  The next ones' loads are in flight behind the work:
-// 4096 rows of 131072 bf16 logits 198 us (5.4 TB/s), 203 us with one at a time.
+// 4096 rows of 131072 bf16 logits 195-200 us (5.4 TB/s), 203 us with one at a time.
 template <int G, typename T, typename F>
 __device__ __forceinline__ void walk(const T* row, int n, int w, int nw, F&& f) {
   const int lane = threadIdx.x & 63;
@@ -440,8 +440,10 @@ constexpr int kAhead = 4;                 // stretches a wave takes at a time
 
 // WAVES waves a row, 4 waves (or WAVES, if more) a workgroup.  KEEP > 0: a wave
 // holds its up to KEEP stretches in registers from the one read to the gradient.
-// Bound by memory: 4096 rows of 50001 bf16 logits and their gradient 196 us (4.2
-// TB/s read and written; rows start at odd places), 249 us read twice.
+// Bound by memory: 4096 rows of 50001 bf16 logits and their gradient 193 us (4.2
+// TB/s read and written; rows start at odd places), 249 us read twice; 189 us where a
+// tenth of the rows is ignored.  65536 wide 229 us (4.7 TB/s); 128256, read twice,
+// 640 us (4.9 TB/s of three passes; two would be 409 us at a copy's rate).
 template <typename T, int WAVES, bool TOP, bool GRAD, int KEEP>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
     logprob_kernel(const T* logits, Args a, T* grad) {
@@ -588,7 +590,8 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
 }
 
 // the gradient from a forward pass's lse and entropy: 4 waves take a stretch of
-// 8192 of a row
+// 8192 of a row (4096 rows of bf16 logits: 50001 wide 179 us, 4.6 TB/s; 128256 425
+// us, 4.9 TB/s)
 constexpr int kGradSpan = 8192;
 
 template <typename T>

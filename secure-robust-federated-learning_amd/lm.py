@@ -25,6 +25,10 @@ Everything runs on torch's current stream of the tensors' device and allocates
 through torch's caching allocator.  Tensors given to be written (``out`` and the
 like) get a new version, as torch's own in-place operations give.  There is no CPU
 path.
+
+Inputs that the kernels cannot walk (columns apart, matrices of a slot that are not
+contiguous) are copied on every call: 8 tables of 17 MB, transposed in memory, make a
+lookup of 11 us one of 140 us.
 """
 from __future__ import annotations
 
@@ -397,10 +401,11 @@ def token_logprobs(logits, targets, top=0, entropy=False, ignore_index=-100):
 def token_logprobs_and_grad(logits, targets, grad_logp, grad_entropy=None, top=0, entropy=False, ignore_index=-100,
                             out=None):
     """``token_logprobs`` and the logits' gradient for given row gradients of logp
-    and entropy (float32 (rows,)), in one pass over the logits: a mean loss over n
-    targets is grad_logp = -1 / n.  Rows with an ignored or bad target, or with
-    grad_logp 0, get zeros (beside the entropy's part) whatever their logits are.
-    ``out`` may be the logits (in place)."""
+    and entropy (float32 (rows,)), in one pass over the logits up to a vocabulary of
+    65536 (float32: 32768), in two beyond: a mean loss over n targets is
+    grad_logp = -1 / n.  Rows with an ignored or bad target, or with grad_logp 0, get
+    zeros (beside the entropy's part) whatever their logits are.  ``out`` may be the
+    logits (in place)."""
     if grad_logp is None:
         raise ValueError("grad_logp is needed")
     return _logprobs(logits, targets, top, entropy, ignore_index, grad_logp, grad_entropy, out)

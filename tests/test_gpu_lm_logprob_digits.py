@@ -156,3 +156,23 @@ def test_a_common_offset_changes_nothing():
     value, err = gradient(w, gl, None, torch.float32)
     ref.within("gradient near", gnear, value, err)
     ref.within("gradient far", gfar, value, err)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_entries_without_the_rest(dtype):
+    """The C entries that know lse alone: the same numbers but the rest."""
+    from srfl_amd import _lib
+    R, V = 10, 5003
+    x, t = rows(V, DT[dtype], 4)
+    gl, _ = weights(4)
+    code, stream = {"fp32": 0, "bf16": 1}[dtype], torch.cuda.current_stream().cuda_stream
+    res, grad = lm.token_logprobs_and_grad(x, t, gl, top=2)
+    logp, lse = torch.empty(2, R, device="cuda").unbind(0)
+    tl, ti, g = torch.empty_like(res.top_logp), torch.empty_like(res.top_ids), torch.empty_like(x)
+    _lib.call("sra_token_logprobs", x.data_ptr(), V, code, t.data_ptr(), R, V, -100, 2, logp.data_ptr(), None,
+              lse.data_ptr(), tl.data_ptr(), ti.data_ptr(), gl.data_ptr(), None, g.data_ptr(), V, stream)
+    for a, b in ((logp, res.logp), (lse, res.lse), (tl, res.top_logp), (ti, res.top_ids), (g, grad)):
+        assert torch.equal(a, b)
+    _lib.call("sra_token_logprobs_grad", x.data_ptr(), V, code, t.data_ptr(), R, V, -100, lse.data_ptr(), None,
+              gl.data_ptr(), None, g.data_ptr(), V, stream)
+    assert torch.equal(g, lm.token_logprobs_grad(x, t, lse, gl))
